@@ -1,0 +1,362 @@
+"""The row operators at the head of a language model: layer normalisation, log probabilities of given tokens (with
+the entropy and the best alternatives) and distillation from a teacher's best logits, each as its cases, in plain torch
+operations, through this framework's functions, and from the definition in 64 bits.
+
+A case's ``op`` says which pass it is:
+
+``ln_forward``   y = layer norm of x with a scale and a bias per column
+``ln_train``     the same, with the gradients of x, scale and bias for a given gradient of y
+``lp_score``     log probability of one token per row, entropy of the row, the ``top`` best tokens
+``lp_train``     log probability and entropy, with the gradient of the logits for given gradients of both
+``kd_train``     loss against a teacher's ``k`` best logits per row, with the gradient of the logits
+
+``dtype`` is the type of x, y and the logits, ``params`` that of scale and bias, ``pad`` the columns by which a row of the
+buffer is longer than the row of logits in it (a vocabulary rounded up), ``masked`` the share of the logits that are
+-infinity, ``temperature`` what the logits are divided by.
+"""
+import functools
+
+import torch
+
+own = False
+
+_TYPES = {"float16": torch.float16, "float32": torch.float32}
+_BYTES = {"float16": 2, "float32": 4}
+
+
+def listed():
+    return [
+        # one token of a model being served: nothing but latency
+        {"name": "ln one token", "op": "ln_forward", "dtype": "float16", "params": "float16", "rows": 1, "cols": 1024},
+        # the rows of this repository's softmax benchmark
+        {"name": "ln forward f32", "op": "ln_forward", "dtype": "float32", "params": "float32", "rows": 32768, "cols": 1024},
+        # a small batch of odd shape, as in fine-tuning a small model
+        {"name": "ln train odd", "op": "ln_train", "dtype": "float32", "params": "float32", "rows": 1237, "cols": 769},
+        # a training step of a large model, half precision with weights kept in single precision
+        {"name": "ln train f16", "op": "ln_train", "dtype": "float16", "params": "float32", "rows": 16384, "cols": 4096},
+        # a step over few, long rows
+        {"name": "ln train wide", "op": "ln_train", "dtype": "float16", "params": "float16", "rows": 2048, "cols": 16384},
+        # one token being generated, with the alternatives an interface shows; odd vocabulary, padded buffer
+        {"name": "lp one token", "op": "lp_score", "dtype": "float16", "rows": 1, "cols": 50257, "pad": 47, "top": 20,
+         "masked": 0.0, "temperature": 1.0},
+        # a batch of requests, decoding under a grammar that forbids half of the tokens
+        {"name": "lp decode batch", "op": "lp_score", "dtype": "float16", "rows": 64, "cols": 128000, "pad": 0, "top": 5,
+         "masked": 0.5, "temperature": 0.7},
+        # scoring whole documents
+        {"name": "lp score f32", "op": "lp_score", "dtype": "float32", "rows": 4096, "cols": 32000, "pad": 0, "top": 0,
+         "masked": 0.0, "temperature": 1.0},
+        # a policy-gradient or fine-tuning step over an odd vocabulary
+        {"name": "lp train f16", "op": "lp_train", "dtype": "float16", "rows": 8192, "cols": 50257, "pad": 47,
+         "masked": 0.0, "temperature": 1.0},
+        # distillation of a toy model: latency
+        {"name": "kd train small", "op": "kd_train", "dtype": "float32", "rows": 33, "cols": 1000, "pad": 0, "k": 8,
+         "masked": 0.0, "temperature": 2.0},
+        # distillation steps over a middle-sized and a large vocabulary
+        {"name": "kd train f32", "op": "kd_train", "dtype": "float32", "rows": 2048, "cols": 32000, "pad": 0, "k": 64,
+         "masked": 0.0, "temperature": 2.0},
+        {"name": "kd train f16", "op": "kd_train", "dtype": "float16", "rows": 4096, "cols": 128000, "pad": 0, "k": 100,
+         "masked": 0.0, "temperature": 1.0},
+    ]
+
+
+def draw(rng):
+    def spread(lo, hi):
+        """Spread over the logarithm; one in three rounded down to a multiple of 64."""
+        v = int(round(lo * (hi / lo) ** rng.random()))
+        return max(lo, v // 64 * 64) if rng.random() < 1 / 3 else v
+
+    op = rng.choice(["ln_forward", "ln_train", "lp_score", "lp_train", "kd_train"])
+    dtype = rng.choice(["float16", "float16", "float32"])
+    if op.startswith("ln"):
+        cols = spread(64, 16384)
+        rows = spread(1, max(2, min(32768, (1 << 26) // _BYTES[dtype] // cols)))
+        params = "float32" if dtype == "float32" else rng.choice(["float16", "float32"])
+        return {"op": op, "dtype": dtype, "params": params, "rows": rows, "cols": cols}
+    cols = spread(500, 160000)
+    most = {"lp_score": 1 << 29, "lp_train": 1 << 29, "kd_train": 1 << 30}[op] // _BYTES[dtype] // cols
+    case = {"op": op, "dtype": dtype, "rows": spread(1, max(2, min(8192, most))), "cols": cols,
+            "pad": rng.choice([0, 0, 1, 8, 47]), "masked": rng.choice([0.0, 0.0, 0.5, 0.9]),
+            "temperature": rng.choice([1.0, 1.0, 0.7, 2.0])}
+    if op == "lp_score":
+        case["top"] = rng.choice([0, 1, 5, 20, rng.randint(2, 64)])
+    if op == "kd_train":
+        case["k"] = spread(1, 256)
+    return case
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rows, cols, dtype = case["rows"], case["cols"], _TYPES[case["dtype"]]
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device="cuda", dtype=torch.float32)
+
+    state = {"case": case}
+    if case["op"].startswith("ln"):
+        params = _TYPES[case["params"]]
+        state["x"] = (normal(rows, cols) * 2 + normal(rows, 1)).to(dtype)
+        state["gamma"] = (1 + 0.1 * normal(cols)).to(params)
+        state["beta"] = (0.1 * normal(cols)).to(params)
+        if case["op"] == "ln_train":
+            state["dy"] = normal(rows, cols).to(dtype)
+        return state
+    buffer = torch.empty(rows, cols + case["pad"], device="cuda", dtype=dtype)
+    state["logits"] = buffer[:, :cols]
+    per = max(1, (1 << 27) // cols)         # rows at a time, so that the numbers on the way need little memory
+    for r in range(0, rows, per):
+        part = 3 * normal(min(per, rows - r), cols + case["pad"])
+        if case["masked"]:
+            part[torch.rand(part.shape, generator=g, device="cuda") < case["masked"]] = float("-inf")
+        buffer[r:r + per] = part.to(dtype)
+    # the mean over the rows; half precision is trained with a scaled loss
+    scale = 4096.0 if case["dtype"] == "float16" else 1.0 / rows
+    if case["op"] == "kd_train":
+        k = case["k"]
+        state["teacher"] = (3 + normal(rows, k).abs()).sort(dim=1, descending=True).values
+        state["ids"] = torch.randint(cols, (rows, k), generator=g, device="cuda", dtype=torch.int32)
+        # rows with fewer entries, and padding rows of a batch, which have none
+        few = torch.rand(rows, 1, generator=g, device="cuda")
+        keep = torch.where(few < 0.05, torch.zeros_like(few), torch.where(few < 0.2, few * 5, torch.ones_like(few)))
+        at = torch.arange(k, device="cuda").unsqueeze(0)
+        state["ids"][at >= keep * k] = -1
+        # a teacher's tokens are among those that are allowed; a token that is there twice gets one value
+        at = state["ids"].long().clamp(min=0)
+        state["logits"].scatter_(1, at, (at * 7919 % 1000 / 250 - 2).to(dtype))
+        state["weight"] = scale * torch.rand(rows, generator=g, device="cuda")
+        return state
+    tokens = torch.randint(cols, (rows,), generator=g, device="cuda", dtype=torch.int64)
+    state["logits"].scatter_(1, tokens.unsqueeze(1), (2 + normal(rows, 1)).to(dtype))
+    if rows > 1:                            # padding of a batch: no token
+        tokens[torch.rand(rows, generator=g, device="cuda") < 0.05] = -1
+    state["tokens"] = tokens
+    if case["op"] == "lp_train":
+        state["weight"] = scale * normal(rows)
+        state["bonus"] = torch.full((rows,), 0.01 * scale, device="cuda")
+    return state
+
+
+# ---- the plain form --------------------------------------------------------------------------------
+
+def _ln_plain(s):
+    x, gamma, beta = s["x"].float(), s["gamma"].float(), s["beta"].float()
+    mean = x.mean(dim=1, keepdim=True)
+    xc = x - mean
+    invstd = 1 / torch.sqrt((xc * xc).mean(dim=1, keepdim=True) + 1e-5)
+    xhat = xc * invstd
+    y = (xhat * gamma + beta).to(s["x"].dtype)
+    if "dy" not in s:
+        return {"y": y}
+    dy = s["dy"].float()
+    a = dy * gamma
+    dx = invstd * (a - a.mean(dim=1, keepdim=True) - xhat * (a * xhat).mean(dim=1, keepdim=True))
+    return {"y": y, "dx": dx.to(s["x"].dtype), "dgamma": (dy * xhat).sum(dim=0).to(s["gamma"].dtype),
+            "dbeta": dy.sum(dim=0).to(s["beta"].dtype)}
+
+
+def _softmax_plain(logits, temperature):
+    """(x - max, exp(x - max), sum, log of the sum, whether anything is left in the row); x are the logits over the
+    temperature.  A row of nothing but -infinity has a sum of 0 and no probability anywhere."""
+    x = logits.float() / temperature
+    top = x.amax(dim=1, keepdim=True)
+    left = top != float("-inf")
+    d = x - torch.where(left, top, torch.zeros_like(top))
+    e = torch.exp(d)
+    total = e.sum(dim=1, keepdim=True)
+    return d, e, total, torch.log(total), left
+
+
+def _best_plain(logits, k):
+    """The k best tokens of each row, the lowest index first among equals: one integer per logit whose order is that of
+    the values and then, falling, of the positions."""
+    bits = (logits.float() + 0.0).view(torch.int32).long()
+    order = torch.where(bits < 0, bits ^ 0x7FFFFFFF, bits)
+    order = torch.where(torch.isnan(logits), torch.full_like(order, 0x7FFFFFFF), order)
+    at = torch.arange(logits.shape[1], device=logits.device)
+    return 0xFFFFFFFF - (torch.topk((order << 32) + (0xFFFFFFFF - at), k, dim=1).values & 0xFFFFFFFF)
+
+
+def _lp_plain(s):
+    case, tokens = s["case"], s["tokens"].unsqueeze(1)
+    given = (tokens >= 0)
+    d, e, total, log_total, left = _softmax_plain(s["logits"], case["temperature"])
+    inf = torch.full_like(total, float("inf"))
+    zero = torch.zeros_like(total)
+    logp = torch.where(left, torch.gather(d, 1, tokens.clamp(min=0)) - log_total, -inf)
+    entropy = torch.where(left, log_total - torch.where(e > 0, e * d, torch.zeros_like(e)).sum(dim=1, keepdim=True) / total, zero)
+    out = {"log_prob": torch.where(given, logp, zero).squeeze(1), "entropy": entropy.squeeze(1)}
+    if case.get("top"):
+        out["top_tokens"] = _best_plain(s["logits"], case["top"])
+        out["top_log_probs"] = torch.where(left, torch.gather(d, 1, out["top_tokens"]) - log_total, -inf)
+    if case["op"] == "lp_train":
+        w = torch.where(given, s["weight"].unsqueeze(1), zero)
+        u = s["bonus"].unsqueeze(1)
+        p = e / total
+        dx = -p * (w + u * (torch.where(p > 0, d, torch.zeros_like(d)) - log_total + entropy))
+        dx.scatter_add_(1, tokens.clamp(min=0), w)
+        dx = torch.where(left, dx / case["temperature"], torch.zeros_like(dx))
+        out["dlogits"] = dx.to(s["logits"].dtype)
+    return out
+
+
+def _kd_plain(s):
+    case, ids = s["case"], s["ids"].long()
+    t = case["temperature"]
+    d, e, total, log_total, left = _softmax_plain(s["logits"], t)
+    teacher = torch.where(ids >= 0, s["teacher"].float(), torch.full_like(s["teacher"], float("-inf")))
+    td, te, t_total, t_log_total, t_left = _softmax_plain(teacher, t)
+    q = torch.where(t_left, te / t_total, torch.zeros_like(te))
+    logp = torch.where(left, torch.gather(d, 1, ids.clamp(min=0)) - log_total, torch.full_like(td, float("-inf")))
+    loss = t * t * torch.where(q > 0, q * (td - t_log_total - logp), torch.zeros_like(q)).sum(dim=1)
+    dx = e / total * q.sum(dim=1, keepdim=True)
+    dx.scatter_add_(1, ids.clamp(min=0), -q)
+    dx = torch.where(left, t * s["weight"].unsqueeze(1) * dx, torch.zeros_like(dx))
+    return {"loss": loss, "dlogits": dx.to(s["logits"].dtype)}
+
+
+# ---- through the framework -------------------------------------------------------------------------
+
+@functools.lru_cache(maxsize=None)
+def _compiled(op, dtype, params, top, temperature):
+    """The function that a program compiles once: device arrays in, device arrays out."""
+    import theano_amd as th
+    from theano_amd import tensor as T
+
+    def matrix(dt):
+        return T.TensorType(dt, (False, False))()
+
+    def vector(dt):
+        return T.TensorType(dt, (False,))()
+
+    def build(ins, outs):
+        return th.function(ins, [th.Out(o, device=True) for o in outs])
+
+    x = matrix(dtype)
+    if op.startswith("ln"):
+        gamma, beta = vector(params), vector(params)
+        y = T.nnet.layer_normalization(x, gamma, beta, epsilon=1e-5)[0]
+        if op == "ln_forward":
+            return build([x, gamma, beta], [y])
+        dy = matrix(dtype)
+        return build([x, gamma, beta, dy], [y] + th.grad(None, [x, gamma, beta], known_grads={y: dy}))
+    if op == "kd_train":
+        teacher, ids, weight = matrix("float32"), matrix("int32"), vector("float32")
+        loss = T.nnet.topk_distillation_loss(x, teacher, ids, temperature=temperature)
+        return build([x, teacher, ids, weight], [loss, th.grad(None, x, known_grads={loss: weight})])
+    tokens = vector("int64")
+    outs = list(T.nnet.token_log_probs(x, tokens, n_top=top, temperature=temperature))
+    if op == "lp_score":
+        return build([x, tokens], outs)
+    weight, bonus = vector("float32"), vector("float32")
+    return build([x, tokens, weight, bonus], outs + [th.grad(None, x, known_grads={outs[0]: weight, outs[1]: bonus})])
+
+
+_INPUTS = {"ln_forward": ("x", "gamma", "beta"), "ln_train": ("x", "gamma", "beta", "dy"), "lp_score": ("logits", "tokens"),
+           "lp_train": ("logits", "tokens", "weight", "bonus"), "kd_train": ("logits", "teacher", "ids", "weight")}
+_OUTPUTS = {"ln_forward": ("y",), "ln_train": ("y", "dx", "dgamma", "dbeta"),
+            "lp_score": ("log_prob", "entropy", "top_log_probs", "top_tokens"), "lp_train": ("log_prob", "entropy", "dlogits"),
+            "kd_train": ("loss", "dlogits")}
+
+
+def _own(s):
+    from theano_amd.hip import HipArray
+    case = s["case"]
+    f = _compiled(case["op"], case["dtype"], case.get("params"), case.get("top"), case.get("temperature"))
+    results = f(*[HipArray.from_cuda_array_interface(s[name]) for name in _INPUTS[case["op"]]])
+    return {name: torch.as_tensor(r, device="cuda") for name, r in zip(_OUTPUTS[case["op"]], results)}
+
+
+def run(state):
+    if own:
+        return _own(state)
+    op = state["case"]["op"]
+    return _ln_plain(state) if op.startswith("ln") else _kd_plain(state) if op == "kd_train" else _lp_plain(state)
+
+
+# ---- what a pass cannot do without -----------------------------------------------------------------
+
+def work(case):
+    rows, cols, n = case["rows"], case["cols"], case["rows"] * case["cols"]
+    size = _BYTES[case["dtype"]]
+    if case["op"] == "ln_forward":
+        return {"bytes": 2 * n * size + 2 * cols * _BYTES[case["params"]], "flops": 8 * n}
+    if case["op"] == "ln_train":        # x and dy in, y and dx out
+        return {"bytes": 4 * n * size + 4 * cols * _BYTES[case["params"]], "flops": 20 * n}
+    if case["op"] == "lp_score":
+        return {"bytes": n * size + rows * (8 + 4 + 4 + 12 * case["top"]), "flops": 7 * n}
+    if case["op"] == "lp_train":
+        return {"bytes": 2 * n * size + rows * (8 + 4 * 4), "flops": 14 * n}
+    return {"bytes": 2 * n * size + rows * (8 * case["k"] + 8), "flops": 11 * n}
+
+
+# ---- from the definition, in 64 bits ---------------------------------------------------------------
+
+def _log_softmax_exact(z):
+    """log(exp(z_j) / sum_i exp(z_i)) of each row; -infinity where nothing is left."""
+    best = z.max(dim=1, keepdim=True).values
+    best = best.masked_fill(best == float("-inf"), 0.0)
+    lse = best + (z - best).exp().sum(dim=1, keepdim=True).log()
+    return (z - lse).masked_fill(lse == float("-inf"), float("-inf"))
+
+
+def _exact_ln(s):
+    x, gamma, beta = (s[k].double() for k in ("x", "gamma", "beta"))
+    var, mean = torch.var_mean(x, dim=1, unbiased=False, keepdim=True)
+    std = (var + 1e-5).sqrt()
+    xhat = (x - mean) / std
+    out = {"y": xhat * gamma + beta}
+    if "dy" in s:
+        dy = s["dy"].double()
+        n = x.shape[1]
+        a = dy * gamma
+        out["dx"] = (n * a - a.sum(dim=1, keepdim=True) - xhat * (a * xhat).sum(dim=1, keepdim=True)) / (n * std)
+        out["dgamma"] = (dy * xhat).sum(dim=0)
+        out["dbeta"] = dy.sum(dim=0)
+    return out
+
+
+def _exact_lp(s, rows):
+    case, tokens = s["case"], s["tokens"][rows]
+    z = s["logits"][rows].double() / case["temperature"]
+    logp = _log_softmax_exact(z)
+    p = logp.exp()
+    plogp = torch.where(p > 0, p * logp, 0.0)
+    h = -plogp.sum(dim=1)
+    r = torch.arange(len(tokens), device=tokens.device)
+    have = tokens >= 0
+    at = torch.where(have, tokens, 0)
+    out = {"log_prob": torch.where(have, logp[r, at], 0.0), "entropy": h}
+    if case.get("top"):
+        best = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :case["top"]]
+        out["top_tokens"] = best
+        out["top_log_probs"] = torch.gather(logp, 1, best)
+    if case["op"] == "lp_train":
+        # d log p_t / dz_j = [j = t] - p_j and dH / dz_j = -p_j (log p_j + H)
+        w = torch.where(have, s["weight"][rows].double(), 0.0)
+        dz = -p * w[:, None] - s["bonus"][rows].double()[:, None] * (plogp + p * h[:, None])
+        dz[r, at] += w
+        out["dlogits"] = (dz / case["temperature"]).masked_fill((z == float("-inf")).all(dim=1, keepdim=True), 0.0)
+    return out
+
+
+def _exact_kd(s, rows):
+    t, ids = s["case"]["temperature"], s["ids"][rows].long()
+    z = s["logits"][rows].double() / t
+    logp = _log_softmax_exact(z)
+    logq = _log_softmax_exact((s["teacher"][rows].double() / t).masked_fill(ids < 0, float("-inf")))
+    q = logq.exp()
+    target = torch.zeros_like(z)
+    target.scatter_add_(1, ids.clamp(min=0), q)
+    cross = torch.where(q > 0, q * (logq - torch.gather(logp, 1, ids.clamp(min=0))), 0.0)
+    dz = logp.exp() * q.sum(dim=1, keepdim=True) - target
+    dz = (dz * t * s["weight"][rows].double()[:, None]).masked_fill((z == float("-inf")).all(dim=1, keepdim=True), 0.0)
+    return {"loss": t * t * cross.sum(dim=1), "dlogits": dz}
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["op"].startswith("ln"):
+        return _exact_ln(s)
+    per = max(1, (1 << 27) // case["cols"])
+    parts = [(_exact_kd if case["op"] == "kd_train" else _exact_lp)(s, slice(r, r + per))
+             for r in range(0, case["rows"], per)]
+    return {name: torch.cat([p[name] for p in parts]) for name in parts[0]}
