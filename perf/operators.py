@@ -243,7 +243,7 @@ def _compiled(op, dtype, params, top, temperature):
         loss = T.nnet.topk_distillation_loss(x, teacher, ids, temperature=temperature)
         return build([x, teacher, ids, weight], [loss, th.grad(None, x, known_grads={loss: weight})])
     tokens = vector("int64")
-    outs = list(T.nnet.token_log_probs(x, tokens, n_top=top, temperature=temperature))
+    outs = list(T.nnet.token_log_probs(x, tokens, n_top=top or 0, temperature=temperature))
     if op == "lp_score":
         return build([x, tokens], outs)
     weight, bonus = vector("float32"), vector("float32")
