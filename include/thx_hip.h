@@ -105,6 +105,12 @@ int thx_d2d(void* dst, const void* src, size_t nbytes);
 int thx_fill_bytes(void* dst, int value, size_t nbytes);     /* GpuArray_memset, a fill kernel */
 int thx_sync(void);
 
+/* The library's one stream (a hipStream_t; null when no device can be had): what a program with streams of its own
+ * orders its work against.  thx_check_device_pointer: THX_OK if `ptr` is memory of the library's device, which an array
+ * made elsewhere has to be (the reference wraps such memory with pygpu.gpuarray.from_gpudata). */
+void* thx_stream(void);
+int thx_check_device_pointer(const void* ptr);
+
 /* ---- run-time compilation ----------------------------------------------- */
 
 /* Directory of the on-disk code-object cache (default $THX_CACHE_DIR, else
@@ -246,6 +252,60 @@ int thx_rowchain_call(thx_rowchain* c, const thx_array* ins, const thx_array* ou
  * unit's registers and LDS hold or when there are too few kept indices to occupy the device. */
 int thx_rowchain_set_axes(thx_rowchain* c, int n_axes, const int32_t* axes);
 int thx_rowchain_free(thx_rowchain* c);
+
+/* ---- Row operators of language models ---------------------------------------
+ * No counterparts in the reference; they stand beside its batch normalisation (theano/tensor/nnet/bn.py:79-263) and its
+ * row softmax and cross-entropies (theano/tensor/nnet/nnet.py:411-646, 2053-2102).  An operand of "rows" has shape
+ * [rows..., cols]: any number of leading axes, which must lie at one stride (THX_ERR_UNSUPPORTED otherwise: the caller
+ * copies), columns side by side.  Operands with one value per row have the leading axes as their shape, at one stride.
+ * Results are C-contiguous and lie over no operand.  "acc" below is float32 for float16 / float32 rows and float64 for
+ * float64 rows; all sums and statistics are computed in it.  Kernels are part of the library: nothing is compiled at
+ * run time.  Work on one stream; every call may be recorded.  Calls that pass partial results between launches take a
+ * workspace of at least the size the matching _workspace function gives for the same operands (16-byte aligned, null
+ * where that is 0; its contents mean nothing before or after, and a recording uses the one it was made with). */
+
+/* y = (x - mean) * invstd * gamma + beta per row, mean and invstd = 1 / sqrt(var + epsilon) of each row stored as acc.
+ * x, y: float16 / float32 / float64 rows of one type.  gamma, beta: [cols] of any stride, both of the type of x, or both
+ * float32 beside float16 rows; beta null: none, gamma null (then beta too): plain normalisation. */
+int thx_layernorm_call(const thx_array* x, const thx_array* gamma, const thx_array* beta, double epsilon,
+                       const thx_array* y, const thx_array* mean, const thx_array* invstd, int flags);
+/* dx = invstd * (a - mean(a) - xhat * mean(a * xhat)), a = dy * gamma; dgamma = sum over rows of dy * xhat, dbeta = sum
+ * over rows of dy, in gamma's type; dgamma and dbeta may be null, gamma too (then both are). */
+int thx_layernorm_grad_workspace(const thx_array* x, const thx_array* dgamma, size_t* nbytes);
+int thx_layernorm_grad_call(const thx_array* x, const thx_array* dy, const thx_array* gamma, const thx_array* mean,
+                            const thx_array* invstd, const thx_array* dx, const thx_array* dgamma,
+                            const thx_array* dbeta, void* workspace, size_t workspace_bytes, int flags);
+
+#define THX_MAX_TOP 64        /* alternatives per row of thx_token_logprob_call */
+#define THX_MAX_TEACHER 1024  /* entries per row of thx_topk_distill_call */
+
+/* p = softmax(logits / temperature) per row; log_prob = log p[token] (0 where token < 0, NaN where token >= cols),
+ * entropy = -sum p log p, the n_top largest log p and their columns (int64; of equal logits the lowest column first,
+ * NaN as the largest), stats [rows..., 2] = largest logit m and log2(sum exp((logits - m) / temperature)).  A row of
+ * nothing but -infinity: log probabilities -infinity, entropy 0.  tokens: int32 or int64.  n_top 0: top_* null. */
+int thx_token_logprob_workspace(const thx_array* logits, int n_top, size_t* nbytes);
+int thx_token_logprob_call(const thx_array* logits, const thx_array* tokens, double temperature, int n_top,
+                           const thx_array* log_prob, const thx_array* entropy, const thx_array* top_log_probs,
+                           const thx_array* top_tokens, const thx_array* stats, void* workspace,
+                           size_t workspace_bytes, int flags);
+/* The gradient of the logits for gradients (each may be null) of log_prob, entropy and top_log_probs; stats, entropy and
+ * top_tokens as the forward call wrote them.  A row of nothing but -infinity gets zeros. */
+int thx_token_logprob_grad_call(const thx_array* logits, const thx_array* tokens, const thx_array* stats,
+                                const thx_array* entropy, const thx_array* top_tokens, const thx_array* g_log_prob,
+                                const thx_array* g_entropy, const thx_array* g_top, double temperature,
+                                const thx_array* dlogits, int flags);
+
+/* q = softmax(teacher / temperature) over a row's entries with token >= 0; loss = temperature^2 sum q (log q -
+ * log p[token]); stats [rows..., 4] = m, log2 sum of the logits as above, then the same of the teacher's.  teacher:
+ * float16 / float32 / float64 [rows..., entries], tokens: int32 / int64 of that shape. */
+int thx_topk_distill_workspace(const thx_array* logits, size_t* nbytes);
+int thx_topk_distill_call(const thx_array* logits, const thx_array* teacher, const thx_array* tokens, double temperature,
+                          const thx_array* loss, const thx_array* stats, void* workspace, size_t workspace_bytes,
+                          int flags);
+/* dlogits_j = g_loss * temperature * (p_j sum(q) - sum_k q_k [j = token_k]). */
+int thx_topk_distill_grad_call(const thx_array* logits, const thx_array* teacher, const thx_array* tokens,
+                               const thx_array* stats, const thx_array* g_loss, double temperature,
+                               const thx_array* dlogits, int flags);
 
 /* ---- inspection and timing ------------------------------------------------ */
 

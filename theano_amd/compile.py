@@ -204,6 +204,7 @@ class Function(object):
         keeps those arrays out of non-temporal accesses so that the last-level cache can serve
         the next read (a batch-norm pass over 100 MB of activations after the statistics pass,
         a reduction over an elementwise result that is also an output)."""
+        from .hip import nnet as hip_nnet
         from .hip.ops import HipArrayType
 
         def root(v):   # the array a chain of views looks at
@@ -215,7 +216,8 @@ class Function(object):
             return isinstance(v.type, HipArrayType) and v.type.ndim > 0 and not any(v.type.broadcastable)
 
         kernels = [n for n in self.nodes
-                   if type(n.op).__name__ in ("HipElemwise", "HipElemwiseReduce", "HipCAReduce", "HipRowChain", "HipMaxAndArgmax")]
+                   if type(n.op).__name__ in ("HipElemwise", "HipElemwiseReduce", "HipCAReduce", "HipRowChain", "HipMaxAndArgmax")
+                   or isinstance(n.op, hip_nnet.DEVICE_OPS)]
         later = set()
         for node in reversed(kernels):
             node.tag["reused_in"] = tuple(k for k, i in enumerate(node.inputs) if big(i) and id(root(i)) in later)
@@ -296,6 +298,7 @@ class Function(object):
         from .tensor.basic import ShapeFloat
         from .tensor.elemwise import DimShuffle
         from .tensor import views as V
+        from .hip import nnet as hip_nnet
         from .hip.ops import HipDimShuffle, HipElemwise, HipCAReduce, HipMaxAndArgmax, HostToHip, HipToHost
         inputs = set(id(v) for v in self.fgraph.inputs)
         pure = {}
@@ -312,8 +315,8 @@ class Function(object):
                         2 if isinstance(op, V.IncSubtensor) else 1):
                     res = False             # extents or indices that are run-time values
                 elif isinstance(op, (HostToHip, HipToHost, DimShuffle, HipElemwise, HipCAReduce, HipMaxAndArgmax,
-                                     V.Subtensor, V.IncSubtensor, V.Reshape, V.Alloc, V.Rebroadcast)) or (
-                                         type(op).__name__ == "HipRowChain"):
+                                     V.Subtensor, V.IncSubtensor, V.Reshape, V.Alloc, V.Rebroadcast) +
+                                hip_nnet.DEVICE_OPS) or type(op).__name__ == "HipRowChain":
                     res = all(shape_pure(i) for i in v.owner.inputs if hasattr(i.type, "ndim"))
                 else:
                     res = False

@@ -85,6 +85,10 @@ std::string entry_name(const std::string& functor, const std::string& plan);
 int launch(const Kernel& k, const std::string& plan, unsigned grid, unsigned block,
            const void* params, size_t params_bytes, bool bare = false);
 
+// Launch of a kernel that is compiled into the library, `args` pointing to its arguments: on the library's stream and
+// device whatever the calling thread's current device is, bracketed by events while profiling like `launch`.
+int launch_builtin(const void* kernel, const std::string& plan, dim3 grid, dim3 block, void** args);
+
 // ---- array helpers ----------------------------------------------------------
 int dtype_size(int dtype);
 const char* dtype_ctype(int dtype);

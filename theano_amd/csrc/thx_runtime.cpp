@@ -522,6 +522,29 @@ int launch(const Kernel& k, const std::string& plan_in, unsigned grid, unsigned 
   return THX_OK;
 }
 
+int launch_builtin(const void* kernel, const std::string& plan, dim3 grid, dim3 block, void** args) {
+  Runtime& r = rt();
+  int current = -1;
+  THX_HIP_CHECK(hipGetDevice(&current));
+  if (current != r.device) THX_HIP_CHECK(hipSetDevice(r.device));
+  ProfRec rec;
+  rec.plan = plan;
+  hipError_t e = hipSuccess;
+  if (g_profiling) {
+    if (e == hipSuccess) e = hipEventCreate(&rec.a);
+    if (e == hipSuccess) e = hipEventCreate(&rec.b);
+    if (e == hipSuccess) e = hipEventRecord(rec.a, r.stream);
+  }
+  if (e == hipSuccess) e = hipLaunchKernel(kernel, grid, block, args, 0, r.stream);
+  if (g_profiling && e == hipSuccess) {
+    e = hipEventRecord(rec.b, r.stream);
+    g_prof.push_back(rec);
+  }
+  if (current != r.device) (void)hipSetDevice(current);
+  if (e != hipSuccess) return fail(THX_ERR_HIP, "launch of '%s' failed: %s", plan.c_str(), hipGetErrorString(e));
+  return THX_OK;
+}
+
 __global__ void thx_fill_kernel(unsigned char* dst, unsigned char value, size_t n) {
   const size_t stride = (size_t)gridDim.x * blockDim.x * 16;
   for (size_t i = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) * 16; i < n; i += stride) {
@@ -651,6 +674,25 @@ int thx_fill_bytes(void* dst, int value, size_t nbytes) {
   hipLaunchKernelGGL(thx_fill_kernel, dim3((unsigned)blocks), dim3(256), 0, rt().stream, (unsigned char*)dst,
                      (unsigned char)value, nbytes);
   THX_HIP_CHECK(hipGetLastError());
+  return THX_OK;
+}
+
+void* thx_stream(void) {
+  if (ensure_init()) return nullptr;
+  return (void*)rt().stream;
+}
+
+int thx_check_device_pointer(const void* ptr) {
+  int rc = ensure_init();
+  if (rc) return rc;
+  hipPointerAttribute_t attr;
+  hipError_t e = hipPointerGetAttributes(&attr, ptr);
+  if (e != hipSuccess || attr.type != hipMemoryTypeDevice) {
+    (void)hipGetLastError();
+    return fail(THX_ERR_ARG, "%p is not device memory", ptr);
+  }
+  if (attr.device != rt().device)
+    return fail(THX_ERR_ARG, "%p lies on device %d, the library uses device %d", ptr, attr.device, rt().device);
   return THX_OK;
 }
 

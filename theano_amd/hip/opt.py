@@ -19,6 +19,7 @@ from ..gof import Constant
 from ..tensor import basic as T
 from ..tensor.elemwise import All, Any, CAReduce, CAReduceDtype, DimShuffle, Elemwise
 from ..tensor.type import TensorConstant, TensorType
+from . import nnet as hip_nnet
 from . import views as hip_views
 from .ops import (HipArrayType, HipCAReduce, HipDimShuffle, HipElemwise, HipElemwiseReduce, HipMaxAndArgmax, HipToHost,
                   HostToHip,
@@ -98,7 +99,7 @@ def lift_to_hip(fgraph):
         ins = [mapped(i) for i in node.inputs]
         op = node.op
         if isinstance(op, (HipElemwise, HipCAReduce, HipMaxAndArgmax, HipDimShuffle, HostToHip, HipToHost, T.ShapeFloat) +
-                      hip_views.DEVICE_OPS):
+                      hip_views.DEVICE_OPS + hip_nnet.DEVICE_OPS):
             if isinstance(op, HostToHip) and isinstance(ins[0].type, HipArrayType):
                 outs = [ins[0]]
             elif isinstance(op, HipToHost):
@@ -123,7 +124,8 @@ def lift_to_hip(fgraph):
             outs = HipMaxAndArgmax(op.axis).make_node(ins[0]).outputs
         elif type(op) in hip_views.LIFT:
             outs = hip_views.LIFT[type(op)](op).make_node(*ins).outputs
-
+        elif type(op) in hip_nnet.LIFT:
+            outs = hip_nnet.LIFT[type(op)](op).make_node(*ins).outputs
         else:
             raise NotImplementedError("%s has no HIP implementation and nothing runs on the host" % op)
         for o, no in zip(node.outputs, outs):

@@ -45,6 +45,7 @@ def _load():
     lib = ctypes.CDLL(_LIB_PATH)
     vp, sz, i32, i64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32, ctypes.c_int64
     P = ctypes.POINTER
+    A = P(thx_array)
     sigs = {
         "thx_init": ([ctypes.c_int], ctypes.c_int),
         "thx_device_info": ([ctypes.c_char_p, sz, P(ctypes.c_int), P(i64)], ctypes.c_int),
@@ -58,6 +59,8 @@ def _load():
         "thx_d2d": ([vp, vp, sz], ctypes.c_int),
         "thx_fill_bytes": ([vp, ctypes.c_int, sz], ctypes.c_int),
         "thx_sync": ([], ctypes.c_int),
+        "thx_stream": ([], vp),
+        "thx_check_device_pointer": ([vp], ctypes.c_int),
         "thx_set_cache_dir": ([ctypes.c_char_p], ctypes.c_int),
         "thx_cache_stats": ([P(i64), P(i64), P(i64)], ctypes.c_int),
         "thx_elemwise_new": ([ctypes.c_char_p, ctypes.c_char_p, ctypes.c_int, ctypes.c_int, P(i32), P(vp)], ctypes.c_int),
@@ -83,6 +86,15 @@ def _load():
         "thx_capture_end": ([P(vp)], ctypes.c_int),
         "thx_graph_launch": ([vp], ctypes.c_int),
         "thx_graph_free": ([vp], ctypes.c_int),
+        "thx_layernorm_call": ([A, A, A, ctypes.c_double, A, A, A, ctypes.c_int], ctypes.c_int),
+        "thx_layernorm_grad_workspace": ([A, A, P(sz)], ctypes.c_int),
+        "thx_layernorm_grad_call": ([A] * 8 + [vp, sz, ctypes.c_int], ctypes.c_int),
+        "thx_token_logprob_workspace": ([A, ctypes.c_int, P(sz)], ctypes.c_int),
+        "thx_token_logprob_call": ([A, A, ctypes.c_double, ctypes.c_int] + [A] * 5 + [vp, sz, ctypes.c_int], ctypes.c_int),
+        "thx_token_logprob_grad_call": ([A] * 8 + [ctypes.c_double, A, ctypes.c_int], ctypes.c_int),
+        "thx_topk_distill_workspace": ([A, P(sz)], ctypes.c_int),
+        "thx_topk_distill_call": ([A] * 3 + [ctypes.c_double, A, A, vp, sz, ctypes.c_int], ctypes.c_int),
+        "thx_topk_distill_grad_call": ([A] * 5 + [ctypes.c_double, A, ctypes.c_int], ctypes.c_int),
         "thx_scratch_reserve": ([sz], ctypes.c_int),
         "thx_scratch_state": ([P(i64), P(i64), P(i64)], ctypes.c_int),
     }
@@ -159,6 +171,13 @@ def device_info():
 
 def sync():
     check(lib.thx_sync())
+
+
+def stream():
+    """The library's one stream as an integer (``hipStream_t``): what a program that uses streams of its own - or
+    another library's, ``torch.cuda.ExternalStream(stream())`` - orders its work against."""
+    init()
+    return lib.thx_stream()
 
 
 def last_plan():
@@ -300,6 +319,18 @@ class _Buffer(object):
             pass
 
 
+class _Foreign(object):
+    """Device memory that another object owns."""
+
+    __slots__ = ("ptr", "owner", "fake")
+
+    def __init__(self, owner, ptr):
+        self.ptr, self.owner, self.fake = ptr, owner, False
+        if not _dry:
+            init()
+            check(lib.thx_check_device_pointer(ptr))
+
+
 def _c_strides(shape, itemsize):
     strides, acc = [], itemsize
     for s in reversed(shape):
@@ -391,6 +422,35 @@ class HipArray(object):
         if a.nbytes and not out.buffer.fake:
             check(lib.thx_h2d(out.buffer.ptr, a.ctypes.data, a.nbytes))
         return out
+
+    @classmethod
+    def from_cuda_array_interface(cls, obj):
+        """A view of device memory that another library holds, through the ``__cuda_array_interface__`` protocol
+        (PyTorch tensors, CuPy arrays): nothing is copied, and ``obj`` lives as long as the view.  The counterpart of
+        ``pygpu.gpuarray.from_gpudata``.  The memory must be the library's device's.  Nothing is ordered here: work on
+        ``obj`` in another stream than ``stream()`` has to be finished, or ordered before that stream, when a function
+        is called on the view."""
+        d = obj.__cuda_array_interface__
+        if d.get("mask") is not None:
+            raise TypeError("a masked array cannot be viewed as a HipArray")
+        dtype, shape, strides = np.dtype(d["typestr"]), tuple(d["shape"]), d.get("strides")
+        if dtype not in _CODE_OF or not dtype.isnative:
+            raise TypeError("dtype %s is not supported on the device" % dtype)
+        if len(shape) > THX_MAX_ND:
+            raise TypeError("arrays of rank %d exceed the limit of %d" % (len(shape), THX_MAX_ND))
+        if 0 in shape:
+            return cls.empty(shape, dtype)
+        strides = _c_strides(shape, dtype.itemsize) if strides is None else tuple(strides)
+        return cls._raw(_Foreign(obj, d["data"][0]), 0, shape, strides, dtype, _CODE_OF[dtype])
+
+    @property
+    def __cuda_array_interface__(self):
+        """The view other libraries take of this array without a copy (``torch.as_tensor(a, device="cuda")``).  They
+        have to order their work after the work in ``stream()``, which the entry ``stream`` names."""
+        if self.dtype.kind == "V" or self.buffer.fake:
+            raise AttributeError("__cuda_array_interface__")
+        return {"shape": self.shape, "typestr": self.dtype.str, "data": (self.ptr if self.size else 0, False),
+                "strides": None if self.c_contiguous else self.strides, "version": 3, "stream": lib.thx_stream()}
 
     # -- properties
     @property

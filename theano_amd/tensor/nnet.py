@@ -886,3 +886,8 @@ def batch_normalization_test(inputs, gamma, beta, mean, var, axes="per-activatio
         raise ValueError("epsilon must be at least 1e-5, got %s" % str(epsilon))
     params, _ = _bn_params(x.type.ndim, axes, [gamma, beta, mean, var], ["gamma", "beta", "mean", "var"])
     return AbstractBatchNormInference(axes)(x, *params, np.asarray(epsilon, dtype=T.config.floatX))
+
+
+from .nnet_lm import (LayerNormalization, LayerNormalizationGrad, TokenLogProbs, TokenLogProbsGrad,  # noqa: F401,E402
+                      TopKDistillation, TopKDistillationGrad, layer_normalization, token_log_probs,
+                      topk_distillation_loss)
