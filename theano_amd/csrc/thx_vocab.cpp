@@ -21,10 +21,17 @@ THX_DEV double acc_exp2(double v) { return exp2(v); }
 THX_DEV float acc_log2(float v) { return log2f(v); }
 THX_DEV double acc_log2(double v) { return log2(v); }
 
+// The rounded product: never the first half of a fused multiply-add.
+template <class A>
+THX_DEV A product(A a, A b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 // c * (x - m).  Half precision: one fused multiply-add against the rounded product c * m, which is the same number
 // wherever the row is read, so that its rounding changes no probability; the products of single precision can overflow
 // (a mask of the type's lowest value), their difference is taken first.
-THX_DEV float scaled(thx_f16 x, float m, float c) { return __builtin_fmaf((float)x, c, -(m * c)); }
+THX_DEV float scaled(thx_f16 x, float m, float c) { return __builtin_fmaf((float)x, c, -product(m, c)); }
 THX_DEV float scaled(float x, float m, float c) { return (x - m) * c; }
 THX_DEV double scaled(double x, double m, double c) { return (x - m) * c; }
 
@@ -47,189 +54,510 @@ THX_DEV A load_real(const void* p, int dtype, int64_t i) {
 // equal logits the lower column.
 typedef unsigned __int128 Wide;
 template <class T> struct Order {
-  typedef unsigned long long Key;
-  THX_DEV static Key key(T v, int64_t col) {
-    const float f = (float)v + 0.0f;
-    unsigned b = __float_as_uint(f);
-    b = f != f ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-    return ((Key)b << 32) | (unsigned)(0xffffffffu - (unsigned)col);
+  typedef unsigned Value;
+  typedef unsigned long long Key;  // value, then 2^32 - 1 - column
+  THX_DEV static Value value(float v) {
+    const float f = v + 0.0f;
+    const unsigned b = __float_as_uint(f);
+    return f != f ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
   }
+  THX_DEV static float inverse(Value v) { return __uint_as_float((v & 0x80000000u) ? v & 0x7fffffffu : ~v); }
+  THX_DEV static Value value_of(Key k) { return (Value)(k >> 32); }
+  THX_DEV static Key key(T v, int64_t col) { return ((Key)value((float)v) << 32) | (unsigned)(0xffffffffu - (unsigned)col); }
+  THX_DEV static Key nan_key(int64_t col) { return ((Key)0xffffffffu << 32) | (unsigned)(0xffffffffu - (unsigned)col); }
 };
 template <> struct Order<double> {
+  typedef unsigned long long Value;
   typedef Wide Key;
-  THX_DEV static Key key(double v, int64_t col) {
+  THX_DEV static Value value(double v) {
     const double f = v + 0.0;
-    unsigned long long b = (unsigned long long)__double_as_longlong(f);
-    b = f != f ? ~0ull : (b >> 63) ? ~b : b | (1ull << 63);
-    return ((Key)b << 32) | (unsigned)(0xffffffffu - (unsigned)col);
+    const unsigned long long b = (unsigned long long)__double_as_longlong(f);
+    return f != f ? ~0ull : (b >> 63) ? ~b : b | (1ull << 63);
   }
+  THX_DEV static double inverse(Value v) { return __longlong_as_double((long long)((v >> 63) ? v & ~(1ull << 63) : ~v)); }
+  THX_DEV static Value value_of(Key k) { return (Value)(k >> 32); }
+  THX_DEV static Key key(double v, int64_t col) { return ((Key)value(v) << 32) | (unsigned)(0xffffffffu - (unsigned)col); }
+  THX_DEV static Key nan_key(int64_t col) { return ((Key)~0ull << 32) | (unsigned)(0xffffffffu - (unsigned)col); }
 };
 template <class Key> THX_DEV int64_t key_column(Key k) { return (int64_t)(0xffffffffu - (unsigned)k); }
 
-template <class A, class F>
-THX_DEV A block_fold(A v, A* lds, F f) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v = f(v, (A)__shfl_xor(v, m, 64));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x / 64] = v;
-  __syncthreads();
-  A r = lds[0];
-  for (unsigned w = 1; w < blockDim.x / 64; ++w) r = f(r, lds[w]);
-  return r;
-}
-struct Plus { template <class A> THX_DEV A operator()(A a, A b) const { return a + b; } };
-struct Most { template <class A> THX_DEV A operator()(A a, A b) const { return a > b ? a : b; } };
+// ---- one wave over a part of a row ----------------------------------------------------------------------------------
+//
+// A part of a row is read once, 64 lanes x kUnroll vectors of 16 bytes at a time.  Each lane keeps the largest logit m
+// of its columns and the sums s = sum 2^d and w = sum d 2^d with d = scaled(x, m); they are rescaled when m grows, which
+// soon happens rarely.  While m is -infinity the exponents are taken against 0: all of them are 0, or NaN, which stays.
 
-// Largest logit and sums of a row; every thread of the block gets them.
-template <class A> struct Sums { A m, s, w; };  // max, sum 2^d, sum d 2^d with d = scaled(x, m)
+constexpr int kUnroll = 4;
+constexpr int kWaves = 4;     // waves of a block; each works alone
+constexpr int kList = 512;    // candidates a wave can hold
+template <class T> struct Width { enum { value = 16 / (int)sizeof(T) }; };
 
-template <class T, class A>
-THX_DEV Sums<A> row_sums(const T* x, int64_t cols, A c, A* lds) {
-  A m = neg_inf<A>();
-  for (int64_t j = threadIdx.x; j < cols; j += blockDim.x) m = Most()(m, (A)x[j]);
-  m = block_fold(m, lds, Most());
-  const A ref = m == neg_inf<A>() ? (A)0 : m;
-  A s = 0, w = 0;
-  for (int64_t j = threadIdx.x; j < cols; j += blockDim.x) {
-    const A d = scaled(x[j], ref, c), e = acc_exp2(d);
-    s += e;
-    w += e * (d < (A)-30000 ? (A)-30000 : d);
+template <class T, bool ENT>
+struct LaneSums {
+  typedef typename AccOf<T>::type A;
+  A m, s, w;
+  A ref;  // what the exponents are taken against: m * c for half precision, else m; 0 while m is -infinity
+  THX_DEV void init() {
+    m = neg_inf<A>();
+    s = w = ref = 0;
   }
-  Sums<A> r;
-  r.m = m;
-  r.s = block_fold(s, lds, Plus());
-  r.w = block_fold(w, lds, Plus());
-  return r;
+  THX_DEV A exponent(A x, A c) const {
+    if constexpr (sizeof(T) == 2) return __builtin_fmaf(x, c, -ref);
+    else return (x - ref) * c;
+  }
+  // d 2^d is 0 where 2^d is, for d = -infinity as well
+  THX_DEV static float bounded(float d) { return __builtin_fmaxf(d, -30000.0f); }
+  THX_DEV static double bounded(double d) { return __builtin_fmax(d, -30000.0); }
+  THX_DEV void raise(A to, A c) {  // to > m
+    const A old = ref;
+    ref = sizeof(T) == 2 ? product(to, c) : to;
+    // between the references as they were rounded, not between the logits
+    const A d = m == neg_inf<A>() ? neg_inf<A>() : sizeof(T) == 2 ? old - ref : (old - ref) * c, k = acc_exp2(d);
+    m = to;
+    if (ENT) w = k * (w + bounded(d) * s);
+    s *= k;
+  }
+  THX_DEV void add(A x, A c) {
+    const A d = exponent(x, c), e = acc_exp2(d);
+    s += e;
+    if (ENT) w += e * bounded(d);
+  }
+  // Takes in the sums of other columns.
+  THX_DEV void join(A om, A os, A ow, A c) {
+    LaneSums o;
+    o.m = om, o.s = os, o.w = ow;
+    o.ref = om == neg_inf<A>() ? (A)0 : (sizeof(T) == 2 ? product(om, c) : om);
+    if (om > m) raise(om, c);
+    else if (m > om) o.raise(m, c);
+    s += o.s;
+    if (ENT) w += o.w;
+  }
+  THX_DEV void join_lanes(A c) {
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+      const A om = __shfl_xor(m, k, 64), os = __shfl_xor(s, k, 64), ow = ENT ? (A)__shfl_xor(w, k, 64) : (A)0;
+      join(om, os, ow, c);
+    }
+  }
+  // A row of nothing but -infinity (a NaN makes the sum a NaN).
+  THX_DEV bool nothing_left() const { return m == neg_inf<A>() && s == (A)0; }
+  THX_DEV A log2_sum() const { return nothing_left() ? neg_inf<A>() : acc_log2(s); }
+};
+
+// Largest of a vector, NaN left aside.
+typedef _Float16 Half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 Half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 Half2 __attribute__((ext_vector_type(2)));
+THX_DEV float vector_max(const Vec<thx_f16, 8>& v) {
+  const Half8 h = *(const Half8*)&v;
+  const Half4 a = __builtin_elementwise_max(h.lo, h.hi);
+  const Half2 b = __builtin_elementwise_max(a.lo, a.hi);
+  return __builtin_fmaxf((float)b.x, (float)b.y);
+}
+THX_DEV float vector_max(const Vec<float, 4>& v) {
+  return __builtin_fmaxf(__builtin_fmaxf(v.v[0], v.v[1]), __builtin_fmaxf(v.v[2], v.v[3]));
+}
+THX_DEV double vector_max(const Vec<double, 2>& v) { return __builtin_fmax(v.v[0], v.v[1]); }
+
+THX_DEV void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+THX_DEV unsigned lanes_below(unsigned long long mask) {
+  return __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
 }
 
-// A row of nothing but -infinity (a NaN makes the sum a NaN).
-template <class A> THX_DEV bool nothing_left(A m, A s) { return m == neg_inf<A>() && s == (A)0; }
+// ---- the best columns ------------------------------------------------------------------------------------------------
+//
+// The k best columns of a part lie in its k best vectors of 16 bytes, a vector standing for its largest value (and its
+// place: of equal vectors the lower one).  Collecting vectors costs the pass one comparison of the maximum it needs
+// anyway; the columns are picked out of the k vectors at the end.  `reached` is a value that k vectors are known to have:
+// the k-th largest of what the 64 lanes have each seen (k <= 64), taken anew after 1, 2, 4, 8 ... steps; vectors below
+// it are passed over.  What reaches it goes to a list in LDS.  Where equal values fill the list, its k best are kept
+// exactly, and from then on only larger values count (equal ones lie further back in the row).
+template <class T>
+struct Best {
+  typedef typename AccOf<T>::type A;
+  typedef typename Order<T>::Key Key;
+  typedef typename Order<T>::Value Value;
+  Key* list;     // kList entries of this wave
+  int n, k;
+  A reached;     // k vectors have this much
+  A limit;       // what a further vector has to have
+  bool closed;   // the list holds k NaN: nothing is larger
+  THX_DEV void init(Key* l, int top) {
+    list = l;
+    n = 0;
+    k = top;
+    reached = limit = neg_inf<A>();
+    closed = false;
+  }
+  // The k-th largest of the lanes' values, bit by bit.
+  THX_DEV A kth_of_lanes(A v) const {
+    const Value mine = Order<T>::value(v);
+    Value p = 0;
+    for (int b = (int)sizeof(Value) * 8 - 1; b >= 0; --b) {
+      const Value t = p | ((Value)1 << b);
+      if (__popcll(__ballot(mine >= t)) >= k) p = t;
+    }
+    return p ? Order<T>::inverse(p) : neg_inf<A>();
+  }
+  THX_DEV void tighten(A lane_max) {
+    const A l = kth_of_lanes(lane_max);
+    if (l > reached) reached = l;
+    if (l > limit) limit = l;
+  }
+  THX_DEV void append(bool take, Key key) {
+    const unsigned long long mask = __ballot(take);
+    if (take) list[n + (int)lanes_below(mask)] = key;
+    n += __popcll(mask);
+  }
+  // Drops what k vectors are known to exceed.
+  THX_DEV void sweep() {
+    const Value v = Order<T>::value(reached);
+    const int lane = threadIdx.x & 63, had = n;
+    n = 0;
+    for (int i = 0; i < had; i += 64) {
+      wave_fence();
+      const Key key = i + lane < had ? list[i + lane] : (Key)0;
+      wave_fence();
+      append(i + lane < had && Order<T>::value_of(key) >= v, key);
+    }
+    wave_fence();
+  }
+  // Puts the largest `keep` entries to the front in falling order.
+  THX_DEV void sort(int keep) {
+    const int lane = threadIdx.x & 63;
+    Key key[kList / 64];
+    int rank[kList / 64];
+#pragma unroll
+    for (int i = 0; i < kList / 64; ++i) {
+      key[i] = i * 64 + lane < n ? list[i * 64 + lane] : (Key)0;
+      rank[i] = 0;
+    }
+    const int used = (n + 63) / 64;
+    for (int j = 0; j < n; ++j) {
+      const Key other = list[j];
+#pragma unroll
+      for (int i = 0; i < kList / 64; ++i)
+        if (i < used) rank[i] += other > key[i];
+    }
+    wave_fence();
+#pragma unroll
+    for (int i = 0; i < kList / 64; ++i)
+      if (i * 64 + lane < n && rank[i] < keep) list[rank[i]] = key[i];
+    wave_fence();
+    n = n < keep ? n : keep;
+  }
+  // Room for `more` entries.
+  THX_DEV void make_room(int more, A lane_max) {
+    if (n + more <= kList) return;
+    tighten(lane_max);
+    sweep();
+    if (n + more <= kList) return;
+    sort(k);
+    const Value v = Order<T>::value_of(list[k - 1]);
+    if (v == (Value)~(Value)0) closed = true;
+    else limit = Order<T>::inverse(v + 1);  // the next larger value (NaN above infinity: no comparison holds)
+  }
+};
+
+// The sums of the vectors [lo, hi) of a row, and its best vectors.
+template <class T, bool ENT, bool TOP>
+THX_DEV void read_part(const T* x, int64_t cols, int64_t lo, int64_t hi, typename AccOf<T>::type c, LaneSums<T, ENT>& sum,
+                       Best<T>& best) {
+  typedef typename AccOf<T>::type A;
+  constexpr int V = Width<T>::value;
+  const int lane = threadIdx.x & 63;
+  const int64_t whole = cols / V;  // vectors that are not cut off by the end of the row
+  sum.init();
+  int steps = 0, next = 1;
+  for (int64_t at = lo; at < hi; at += 64 * kUnroll) {
+    Vec<T, V> v[kUnroll];
+    if (at + 64 * kUnroll <= hi && at + 64 * kUnroll <= whole) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) load_vec<T, V, false, true>(v[u], x + (at + u * 64 + lane) * V);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t i = at + u * 64 + lane;
+        if (i < hi && i < whole) {
+          load_vec<T, V, false, true>(v[u], x + i * V);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[u].v[e] = i < hi && i * V + e < cols ? x[i * V + e] : (T)neg_inf<A>();
+        }
+      }
+    }
+    A vm[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) vm[u] = vector_max(v[u]);
+    A m = vm[0];
+#pragma unroll
+    for (int u = 1; u < kUnroll; ++u) m = m > vm[u] ? m : vm[u];
+    if (m > sum.m) sum.raise(m, c);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum.add((A)v[u].v[e], c);
+    if constexpr (TOP) {
+      if (++steps == next) {
+        best.tighten(sum.m);
+        next *= 2;
+      }
+      const bool odd = sum.s != sum.s;  // NaN (or +infinity) somewhere in this lane's columns
+      if (__ballot(m >= best.limit || odd) && !best.closed) {
+        best.make_room(64 * kUnroll, sum.m);
+        if (!best.closed) {
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u) {
+            const int64_t i = at + u * 64 + lane;
+            bool nan = false;
+            if (odd) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) nan |= v[u].v[e] != v[u].v[e];
+            }
+            best.append(i < hi && (vm[u] >= best.limit || nan),
+                        nan ? Order<T>::nan_key(i) : Order<T>::key((T)vm[u], i));
+          }
+          wave_fence();
+        }
+      }
+    }
+  }
+  if constexpr (TOP) {
+    best.tighten(sum.m);
+    best.sweep();
+    best.sort(best.k);
+  }
+}
+
+// ---- results of a row, by one wave -------------------------------------------------------------------------------------
 
 template <class A> struct LpOut { A *log_prob, *entropy, *top; int64_t* top_at; A* stats; };
 
 template <class T>
-__global__ void __launch_bounds__(256) lp_forward(const T* x, int64_t xs, int64_t rows, int64_t cols, const void* tokens,
-                                                  int64_t ts, int t64, typename AccOf<T>::type c,
-                                                  typename AccOf<T>::type inv_t, int n_top, LpOut<typename AccOf<T>::type> o) {
+struct LpRow {  // what lp_forward needs besides the logits
+  typedef typename AccOf<T>::type A;
+  const void* tokens;
+  int64_t ts;
+  int t64, n_top;
+  A inv_t;
+  LpOut<A> o;
+};
+
+// The best columns out of the best vectors (in best.list, falling), and everything else of the row; `sum` joined.
+template <class T, bool TOP>
+THX_DEV void finish(const LpRow<T>& q, const T* x, int64_t cols, int64_t r, typename AccOf<T>::type c,
+                    const LaneSums<T, true>& sum, Best<T>& best) {
   typedef typename AccOf<T>::type A;
   typedef typename Order<T>::Key Key;
-  __shared__ A lds[4];
-  __shared__ Key best[4];
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T* xr = x + r * xs;
-    const Sums<A> q = row_sums<T, A>(xr, cols, c, lds);
-    const bool none = nothing_left(q.m, q.s);
-    const A ls = none ? neg_inf<A>() : acc_log2(q.s);
-    if (threadIdx.x == 0) {
-      const int64_t t = load_index(tokens, t64, r * ts);
-      A lp = 0;
-      if (t >= cols) lp = (A)NAN;
-      else if (t >= 0) lp = none ? neg_inf<A>() : log_prob(xr[t], q.m, c, inv_t, ls);
-      o.log_prob[r] = lp;
-      o.entropy[r] = none ? (A)0 : (ls - q.w / q.s) * (A)kLn2;
-      o.stats[2 * r] = q.m;
-      o.stats[2 * r + 1] = ls;
-    }
-    Key last = ~(Key)0;  // no column has this key: a column of 0 would need 2^32 - 1 less it
-    bool first = true;
-    for (int k = 0; k < n_top; ++k) {
-      Key b = 0;
-      for (int64_t j = threadIdx.x; j < cols; j += blockDim.x) {
-        const Key v = Order<T>::key(xr[j], j);
-        if ((first || v < last) && v > b) b = v;
-      }
-      for (int m = 32; m >= 1; m >>= 1) {
-        Key other;
-        unsigned* w = (unsigned*)&other;
-        const unsigned* mine = (const unsigned*)&b;
-        for (int i = 0; i < (int)(sizeof(Key) / 4); ++i) w[i] = (unsigned)__shfl_xor((int)mine[i], m, 64);
-        if (other > b) b = other;
-      }
-      __syncthreads();
-      if ((threadIdx.x & 63) == 0) best[threadIdx.x / 64] = b;
-      __syncthreads();
-      for (int w = 0; w < 4; ++w)
-        if (best[w] > b) b = best[w];
-      last = b;
-      first = false;
-      if (threadIdx.x == 0) {
-        const int64_t j = key_column(b);
-        o.top_at[r * n_top + k] = j;
-        o.top[r * n_top + k] = none ? neg_inf<A>() : log_prob(xr[j], q.m, c, inv_t, ls);
-      }
-    }
-    __syncthreads();
+  constexpr int V = Width<T>::value;
+  const int lane = threadIdx.x & 63;
+  const bool none = sum.nothing_left();
+  const A ls = sum.log2_sum();
+  if (lane == 0) {
+    const int64_t t = load_index(q.tokens, q.t64, r * q.ts);
+    A lp = 0;
+    if (t >= cols) lp = (A)NAN;
+    else if (t >= 0) lp = none ? neg_inf<A>() : log_prob(x[t], sum.m, c, q.inv_t, ls);
+    q.o.log_prob[r] = lp;
+    q.o.entropy[r] = none ? (A)0 : (ls - sum.w / sum.s) * (A)kLn2;
+    q.o.stats[2 * r] = sum.m;
+    q.o.stats[2 * r + 1] = ls;
   }
-}
-
-// Teacher's side of one row: largest logit and sum over the entries there are; every thread gets them.
-template <class A>
-THX_DEV void teacher_sums(const void* teacher, int tdt, const void* ids, int i64, int64_t t0, int64_t i0, int n, A c, A* lds,
-                          A& m, A& s) {
-  m = neg_inf<A>();
-  for (int k = threadIdx.x; k < n; k += blockDim.x)
-    if (load_index(ids, i64, i0 + k) >= 0) m = Most()(m, load_real<A>(teacher, tdt, t0 + k));
-  m = block_fold(m, lds, Most());
-  s = 0;
-  for (int k = threadIdx.x; k < n; k += blockDim.x)
-    if (load_index(ids, i64, i0 + k) >= 0)
-      s += acc_exp2((load_real<A>(teacher, tdt, t0 + k) - (m == neg_inf<A>() ? (A)0 : m)) * c);
-  s = block_fold(s, lds, Plus());
+  if constexpr (TOP) {
+    const int vectors = best.n, k = best.k;  // fewer vectors than k: all there are
+    const Key least = vectors >= k ? best.list[k - 1] : (Key)0;
+    constexpr int kMost = THX_MAX_TOP * V / 64;
+    Key key[kMost];
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      const int e = i * 64 + lane;  // element e % V of vector e / V
+      key[i] = 0;
+      if (e < vectors * V) {
+        const int64_t j = key_column(best.list[e / V]) * V + e % V;
+        if (j < cols) key[i] = Order<T>::key(x[j], j);
+      }
+    }
+    wave_fence();
+    best.n = 0;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i)
+      best.append(key[i] != (Key)0 && Order<T>::value_of(key[i]) >= Order<T>::value_of(least), key[i]);
+    wave_fence();
+    best.sort(k);
+    if (lane < k) {
+      const int64_t j = key_column(best.list[lane]);
+      q.o.top_at[r * k + lane] = j;
+      q.o.top[r * k + lane] = none ? neg_inf<A>() : log_prob(x[j], sum.m, c, q.inv_t, ls);
+    }
+  }
 }
 
 template <class A> struct Teacher { const void* logits; int64_t ls; int dtype; const void* ids; int64_t is; int i64, n; };
 
 template <class T>
-__global__ void __launch_bounds__(256) kd_forward(const T* x, int64_t xs, int64_t rows, int64_t cols,
-                                                  Teacher<typename AccOf<T>::type> t, typename AccOf<T>::type c,
-                                                  typename AccOf<T>::type inv_t, typename AccOf<T>::type t2,
-                                                  typename AccOf<T>::type* loss,
-                                                  typename AccOf<T>::type* stats) {
+struct KdRow {
   typedef typename AccOf<T>::type A;
-  __shared__ A lds[4];
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T* xr = x + r * xs;
-    const Sums<A> q = row_sums<T, A>(xr, cols, c, lds);
-    const bool none = nothing_left(q.m, q.s);
-    const A ls = none ? neg_inf<A>() : acc_log2(q.s);
-    A tm, ts;
-    teacher_sums<A>(t.logits, t.dtype, t.ids, t.i64, r * t.ls, r * t.is, t.n, c, lds, tm, ts);
-    const bool tnone = nothing_left(tm, ts);
-    const A tls = tnone ? neg_inf<A>() : acc_log2(ts);
-    A sum = 0;
-    for (int k = threadIdx.x; k < t.n; k += blockDim.x) {
-      const int64_t id = load_index(t.ids, t.i64, r * t.is + k);
-      if (id < 0) continue;
-      if (id >= cols) sum = (A)NAN;
-      if (id >= cols || tnone) continue;
-      const A tv = load_real<A>(t.logits, t.dtype, r * t.ls + k), p = acc_exp2((tv - tm) * c - tls);
-      const A lp = none ? neg_inf<A>() : log_prob(xr[id], q.m, c, inv_t, ls);
-      if (!(p == (A)0)) sum += p * (log_prob(tv, tm, c, inv_t, tls) - lp);
-    }
-    sum = block_fold(sum, lds, Plus());
-    if (q.s != q.s) sum = q.s;
-    if (threadIdx.x == 0) {
-      loss[r] = sum * t2;
-      stats[4 * r] = q.m;
-      stats[4 * r + 1] = ls;
-      stats[4 * r + 2] = tm;
-      stats[4 * r + 3] = tls;
-    }
-    __syncthreads();
+  Teacher<A> t;
+  A inv_t, t2;
+  A *loss, *stats;
+};
+
+template <class T>
+THX_DEV void finish(const KdRow<T>& q, const T* x, int64_t cols, int64_t r, typename AccOf<T>::type c,
+                    const LaneSums<T, false>& sum) {
+  typedef typename AccOf<T>::type A;
+  const Teacher<A>& t = q.t;
+  const int lane = threadIdx.x & 63;
+  const bool none = sum.nothing_left();
+  const A ls = sum.log2_sum();
+  LaneSums<A, false> ts;  // the teacher's side: entries as single or double precision
+  ts.init();
+  for (int k = lane; k < t.n; k += 64) {
+    if (load_index(t.ids, t.i64, r * t.is + k) < 0) continue;
+    const A v = load_real<A>(t.logits, t.dtype, r * t.ls + k);
+    if (v > ts.m) ts.raise(v, c);
+    ts.add(v, c);
+  }
+  ts.join_lanes(c);
+  const bool tnone = ts.nothing_left();
+  const A tls = ts.log2_sum();
+  A loss = 0;
+  for (int k = lane; k < t.n; k += 64) {
+    const int64_t id = load_index(t.ids, t.i64, r * t.is + k);
+    if (id < 0) continue;
+    if (id >= cols) loss = (A)NAN;
+    if (id >= cols || tnone) continue;
+    const A v = load_real<A>(t.logits, t.dtype, r * t.ls + k), p = acc_exp2((v - ts.m) * c - tls);
+    const A lp = none ? neg_inf<A>() : log_prob(x[id], sum.m, c, q.inv_t, ls);
+    if (!(p == (A)0)) loss += p * (log_prob(v, ts.m, c, q.inv_t, tls) - lp);
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) loss += __shfl_xor(loss, k, 64);
+  if (sum.s != sum.s) loss = sum.s;
+  if (lane == 0) {
+    q.loss[r] = loss * q.t2;
+    q.stats[4 * r] = sum.m;
+    q.stats[4 * r + 1] = ls;
+    q.stats[4 * r + 2] = ts.m;
+    q.stats[4 * r + 3] = tls;
   }
 }
 
-// dx_j = p_j (a + b log2 p_j) + sum_k c_k [j = id_k]: the gradient of every function of the log probabilities above.
-template <class T, class A>
-THX_DEV void grad_row(const T* xr, T* dr, int64_t cols, A m, A ls, A c, A a, A b) {
-  const bool none = m == neg_inf<A>() && ls == neg_inf<A>();
-  for (int64_t j = threadIdx.x; j < cols; j += blockDim.x) {
-    const A l = scaled(xr[j], none ? (A)0 : m, c) - ls, p = acc_exp2(l);
-    A v = p * a;
-    if (b != (A)0) v += p * b * (l < (A)-30000 ? (A)-30000 : l);
-    dr[j] = none ? (T)0 : (T)v;
+// ---- forward kernels ---------------------------------------------------------------------------------------------------
+
+// The rows of a call and how they are cut: `parts` waves to a row, `per` vectors to a part.  A row of several parts leaves
+// its sums in partial[row][part][3] and its best vectors (k of them, 0 for none) in lists[row][part][k].
+template <class T>
+struct Cut {
+  typedef typename AccOf<T>::type A;
+  const T* x;
+  int64_t xs, rows, cols;
+  int64_t per;
+  int parts;
+  A c;
+  A* partial;
+  typename Order<T>::Key* lists;
+};
+
+template <class T, bool TOP, class Row, bool ENT>
+__global__ void __launch_bounds__(64 * kWaves) vocab_read(Cut<T> q, Row row) {
+  typedef typename Order<T>::Key Key;
+  constexpr int V = Width<T>::value;
+  __shared__ Key lists[TOP ? kWaves * kList : 1];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+  const int64_t units = q.rows * q.parts, vectors = (q.cols + V - 1) / V;
+  for (int64_t unit = (int64_t)blockIdx.x * kWaves + wave; unit < units; unit += (int64_t)gridDim.x * kWaves) {
+    const int64_t r = unit / q.parts, part = unit - r * q.parts;
+    const T* x = q.x + r * q.xs;
+    const int64_t lo = part * q.per, hi = lo + q.per < vectors ? lo + q.per : vectors;
+    LaneSums<T, ENT> sum;
+    Best<T> best;
+    int k = 0;
+    if constexpr (TOP) {
+      k = row.n_top;
+      best.init(lists + wave * kList, k);
+    }
+    read_part<T, ENT, TOP>(x, q.cols, lo, hi, q.c, sum, best);
+    sum.join_lanes(q.c);
+    if (q.parts == 1) {
+      if constexpr (ENT) finish<T, TOP>(row, x, q.cols, r, q.c, sum, best);
+      else finish<T>(row, x, q.cols, r, q.c, sum);
+      wave_fence();
+      continue;
+    }
+    if (lane == 0) {
+      auto* p = q.partial + unit * 3;
+      p[0] = sum.m, p[1] = sum.s, p[2] = ENT ? sum.w : 0;
+    }
+    if (lane < k) q.lists[unit * k + lane] = lane < best.n ? best.list[lane] : (Key)0;
+    wave_fence();
   }
 }
+
+// The largest key of the wave.
+template <class Key>
+THX_DEV Key wave_max(Key v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    Key o;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Key) / 4); ++i) ((unsigned*)&o)[i] = (unsigned)__shfl_xor((int)((unsigned*)&v)[i], m, 64);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+
+// One wave per row over its parts (at most 64: one to a lane).
+template <class T, bool TOP, class Row, bool ENT>
+__global__ void __launch_bounds__(64) vocab_join(Cut<T> q, Row row) {
+  typedef typename Order<T>::Key Key;
+  __shared__ Key lists[TOP ? kList : 1];
+  const int lane = threadIdx.x;
+  for (int64_t r = blockIdx.x; r < q.rows; r += gridDim.x) {
+    LaneSums<T, ENT> sum;
+    sum.init();
+    if (lane < q.parts) {
+      const auto* p = q.partial + (r * q.parts + lane) * 3;
+      sum.join(p[0], p[1], p[2], q.c);
+    }
+    sum.join_lanes(q.c);
+    const T* x = q.x + r * q.xs;
+    if constexpr (ENT) {
+      Best<T> best;
+      if constexpr (TOP) {
+        const int k = row.n_top;
+        best.init(lists, k);
+        const Key* mine = q.lists + (r * q.parts + lane) * k;
+        int at = 0;
+        Key head = lane < q.parts ? mine[0] : (Key)0;
+        for (int i = 0; i < k; ++i) {
+          const Key top = wave_max(head);
+          if (top == (Key)0) break;
+          if (lane == 0) best.list[i] = top;
+          best.n = i + 1;
+          if (head == top) {
+            ++at;
+            head = at < k ? mine[at] : (Key)0;
+          }
+        }
+        wave_fence();
+      }
+      finish<T, TOP>(row, x, q.cols, r, q.c, sum, best);
+    } else {
+      finish<T>(row, x, q.cols, r, q.c, sum);
+    }
+    wave_fence();
+  }
+}
+
+// ---- gradient ------------------------------------------------------------------------------------------------------------
+//
+// dx_j = p_j (a + b log2 p_j) + sum_k v_k [j = id_k] is the gradient of every function of the log probabilities above.
+// With d = scaled(x_j, m) and p_j = 2^d / S it is 2^d (a' + b' d) with a' = (a - b log2 S) / S and b' = b / S: one
+// exponential and one rounding of the row's statistics per element.  The columns of the list are few; their elements are
+// written once more, each by the thread of the entry that names the column first, from the sum of all entries that do.
+
+template <class A> struct Slope { A m, ls, a, b; };
 
 template <class A>
 struct LpGrad {
@@ -240,91 +568,200 @@ struct LpGrad {
   const A* g; int64_t gs;
   const A* u; int64_t us;
   const A* gt; int64_t gts;
+  A inv_t;
+
+  THX_DEV int entries() const { return n_top + 1; }
+  // The entries of row r into LDS, and the slope of the rest; called by the whole block.
+  THX_DEV Slope<A> open(int64_t r, int64_t cols, int* id, A* val) const {
+    const A* st = stats + r * ss;
+    const int64_t t = load_index(tokens, t64, r * ts);
+    const A w = g && t >= 0 ? g[r * gs] : (A)0;
+    A a = t >= cols && g ? (A)NAN : w;
+    for (int k = 0; k < n_top; ++k) a += gt[r * gts + k];
+    const A h = u ? u[r * us] : (A)0;
+    if (u) a += h * entropy[r * es];
+    const int k = threadIdx.x;
+    if (k < n_top) {
+      const int64_t j = top[r * ps + k];
+      id[k] = j >= 0 && j < cols ? (int)j : -1;
+      val[k] = gt[r * gts + k] * inv_t;
+    }
+    if (k == n_top) {
+      id[k] = g && t >= 0 && t < cols ? (int)t : -1;
+      val[k] = w * inv_t;
+    }
+    return {st[0], st[1], -a * inv_t, -h * (A)kLn2 * inv_t};
+  }
+};
+
+template <class A>
+struct KdGrad {
+  Teacher<A> t;
+  const A* stats; int64_t ss;
+  const A* g; int64_t gs;
+  A c, temperature;
+
+  THX_DEV int entries() const { return t.n; }
+  THX_DEV Slope<A> open(int64_t r, int64_t cols, int* id, A* val) const {
+    const A* st = stats + r * ss;
+    const A tm = st[2], tls = st[3], gt = g[r * gs] * temperature;
+    const bool tnone = tm == neg_inf<A>() && tls == neg_inf<A>();
+    bool beyond = false;
+    for (int k = threadIdx.x; k < t.n; k += blockDim.x) {
+      const int64_t j = load_index(t.ids, t.i64, r * t.is + k);
+      beyond |= j >= cols;
+      id[k] = j >= 0 && j < cols && !tnone ? (int)j : -1;
+      val[k] = -gt * acc_exp2((load_real<A>(t.logits, t.dtype, r * t.ls + k) - tm) * c - tls);
+    }
+    const bool bad = __syncthreads_or(beyond);
+    return {st[0], st[1], bad ? (A)NAN : tnone ? (A)0 : gt, (A)0};
+  }
 };
 
 template <class T>
-__global__ void __launch_bounds__(256) lp_backward(const T* x, int64_t xs, int64_t rows, int64_t cols,
-                                                   LpGrad<typename AccOf<T>::type> q, typename AccOf<T>::type c,
-                                                   typename AccOf<T>::type inv_t, T* dx) {
+struct GradCut {
   typedef typename AccOf<T>::type A;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T* xr = x + r * xs;
-    T* dr = dx + r * cols;
-    const A m = q.stats[r * q.ss], ls = q.stats[r * q.ss + 1];
-    const bool none = m == neg_inf<A>() && ls == neg_inf<A>();
-    int64_t t = load_index(q.tokens, q.t64, r * q.ts);
-    A w = q.g && t >= 0 ? q.g[r * q.gs] : (A)0;
-    A a = t >= cols && q.g ? (A)NAN : w;
-    if (t >= cols) t = -1;
-    for (int k = 0; k < q.n_top; ++k) a += q.gt[r * q.gts + k];
-    const A u = q.u ? q.u[r * q.us] : (A)0;
-    if (q.u) a += u * q.entropy[r * q.es];
-    grad_row<T, A>(xr, dr, cols, m, ls, c, -a * inv_t, -u * (A)kLn2 * inv_t);
-    __syncthreads();
-    if (none) continue;
-    for (int k = threadIdx.x; k <= q.n_top; k += blockDim.x) {
-      const int64_t id = k == q.n_top ? (q.g ? t : -1) : q.top[r * q.ps + k];
-      if (id < 0 || id >= cols) continue;
-      A v = id == t ? w : (A)0;
-      bool mine = true;
-      for (int i = 0; i < q.n_top; ++i)
-        if (q.top[r * q.ps + i] == id) {
-          v += q.gt[r * q.gts + i];
-          if (i < k) mine = false;
-        }
-      if (!mine) continue;
-      const A l = scaled(xr[id], m, c) - ls, p = acc_exp2(l);
-      A d = -p * a;
-      if (u != (A)0) d -= p * u * (A)kLn2 * (l < (A)-30000 ? (A)-30000 : l);
-      dr[id] = (T)((d + v) * inv_t);
-    }
-  }
-}
+  const T* x;
+  int64_t xs, rows, cols;
+  int64_t per;  // vectors of a segment
+  int segs;     // segments of a row
+  A c;
+  T* dx;
+};
 
-template <class T>
-__global__ void __launch_bounds__(256) kd_backward(const T* x, int64_t xs, int64_t rows, int64_t cols,
-                                                   Teacher<typename AccOf<T>::type> t,
-                                                   const typename AccOf<T>::type* stats, int64_t ss,
-                                                   const typename AccOf<T>::type* g, int64_t gs,
-                                                   typename AccOf<T>::type c, typename AccOf<T>::type temperature, T* dx) {
+template <class T, class Row>
+__global__ void __launch_bounds__(256) vocab_grad(GradCut<T> q, Row row) {
   typedef typename AccOf<T>::type A;
-  __shared__ A lds[4];
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T* xr = x + r * xs;
-    T* dr = dx + r * cols;
-    const A m = stats[r * ss], ls = stats[r * ss + 1], tm = stats[r * ss + 2], tls = stats[r * ss + 3];
-    const bool none = m == neg_inf<A>() && ls == neg_inf<A>();
-    const bool tnone = tm == neg_inf<A>() && tls == neg_inf<A>();
-    const A gt = g[r * gs] * temperature;
-    A bad = 0;
-    for (int k = threadIdx.x; k < t.n; k += blockDim.x)
-      if (load_index(t.ids, t.i64, r * t.is + k) >= cols) bad = (A)1;
-    bad = block_fold(bad, lds, Most());
-    A a = tnone ? (A)0 : gt;
-    if (bad != (A)0) a = (A)NAN;
-    grad_row<T, A>(xr, dr, cols, m, ls, c, a, (A)0);
-    __syncthreads();
-    if (!none && !tnone && bad == (A)0) {
-      for (int k = threadIdx.x; k < t.n; k += blockDim.x) {
-        const int64_t id = load_index(t.ids, t.i64, r * t.is + k);
-        if (id < 0) continue;
-        A v = 0;
-        bool mine = true;
-        for (int i = 0; i < t.n; ++i)
-          if (load_index(t.ids, t.i64, r * t.is + i) == id) {
-            if (i < k) mine = false;
-            v += acc_exp2((load_real<A>(t.logits, t.dtype, r * t.ls + i) - tm) * c - tls);
-          }
-        if (mine) dr[id] = (T)(gt * (acc_exp2(scaled(xr[id], m, c) - ls) - v));
+  constexpr int V = Width<T>::value;
+  __shared__ int id[THX_MAX_TEACHER];
+  __shared__ A val[THX_MAX_TEACHER];
+  const int64_t units = q.rows * q.segs, whole = q.cols / V, vectors = (q.cols + V - 1) / V;
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int64_t r = unit / q.segs, seg = unit - r * q.segs;
+    const T* x = q.x + r * q.xs;
+    T* dx = q.dx + r * q.cols;
+    const Slope<A> s = row.open(r, q.cols, id, val);
+    const bool none = s.m == neg_inf<A>() && s.ls == neg_inf<A>();
+    LaneSums<T, false> at;
+    at.ref = none ? (A)0 : sizeof(T) == 2 ? product(s.m, q.c) : s.m;
+    const A inv = none ? (A)0 : acc_exp2(-s.ls);
+    const A a = none ? (A)0 : (s.a - s.b * s.ls) * inv, b = s.b * inv;
+    const int64_t lo = seg * q.per, hi = lo + q.per < vectors ? lo + q.per : vectors;
+    auto slope = [&](T v) {
+      const A d = at.exponent((A)v, q.c), e = acc_exp2(d);
+      return b == (A)0 ? e * a : e * (a + b * LaneSums<T, false>::bounded(d));
+    };
+    for (int64_t i0 = lo; i0 < hi; i0 += 256 * kUnroll) {
+      Vec<T, V> v[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t i = i0 + u * 256 + threadIdx.x;
+        if (i < hi && i < whole) load_vec<T, V, false, true>(v[u], x + i * V);
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t i = i0 + u * 256 + threadIdx.x;
+        if (i < hi && i < whole) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[u].v[e] = none ? (T)0 : (T)slope(v[u].v[e]);
+          store_vec<T, V, false, true>(dx + i * V, v[u]);
+        } else if (i < hi) {
+          for (int64_t j = i * V; j < q.cols; ++j) dx[j] = none ? (T)0 : (T)slope(x[j]);
+        }
       }
     }
-    __syncthreads();
+    __syncthreads();  // the entries are there, and the elements they replace are written
+    if (!none) {
+      const int n = row.entries();
+      const int64_t first = lo * V, last = hi * V;
+      for (int k = threadIdx.x; k < n; k += 256) {
+        const int j = id[k];
+        if (j < first || j >= last) continue;
+        A v = 0;
+        bool mine = true;
+        for (int i = 0; i < n; ++i)
+          if (id[i] == j) {
+            v += val[i];
+            if (i < k) mine = false;
+          }
+        if (mine) dx[j] = (T)(slope(x[j]) + v);
+      }
+    }
+    __syncthreads();  // before the next row's entries
   }
 }
 
 int acc_code(int dtype) { return dtype == THX_F64 ? THX_F64 : THX_F32; }
 bool is_float(int dtype) { return dtype == THX_F16 || dtype == THX_F32 || dtype == THX_F64; }
 unsigned grid_of(int64_t n) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(n, 1 << 20)); }
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// How a call's rows are cut for the forward pass: enough waves to fill the device, one per row where there are rows enough
+// (nothing to join then), and no more than 64 parts, each of at least one step of a wave.
+int parts_of(int64_t rows, int64_t vectors) {
+  const int64_t want = ceil_div((int64_t)compute_units() * 16, std::max<int64_t>(rows, 1));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, 64, ceil_div(vectors, 64)}));
+}
+
+// Sums, then lists, of all parts.
+size_t partial_bytes(const Rows& x, int n_top) {
+  const int isz = dtype_size(x.dtype);
+  const int64_t parts = parts_of(x.rows, ceil_div(x.cols * isz, 16));
+  if (parts == 1 || !x.rows) return 0;
+  const int acc = dtype_size(acc_code(x.dtype));
+  const size_t sums = ((size_t)x.rows * parts * 3 * acc + 15) / 16 * 16;
+  return sums + (size_t)x.rows * parts * n_top * (acc == 8 ? 16 : 8);
+}
+
+std::string plan_of(const char* name, const Rows& x) {
+  return std::string(name) + "|t" + std::to_string(x.dtype) + "|p" +
+         std::to_string(parts_of(x.rows, ceil_div(x.cols * dtype_size(x.dtype), 16)));
+}
+
+template <class T>
+Cut<T> cut_of(const Rows& x, double temperature, void* ws) {
+  typedef typename AccOf<T>::type A;
+  Cut<T> q;
+  const int64_t vectors = ceil_div(x.cols, Width<T>::value);
+  q.x = (const T*)x.ptr;
+  q.xs = x.stride, q.rows = x.rows, q.cols = x.cols;
+  q.parts = parts_of(x.rows, vectors);
+  q.per = ceil_div(vectors, q.parts);
+  q.c = (A)(kLog2E / temperature);
+  q.partial = (A*)ws;
+  q.lists = (typename Order<T>::Key*)((char*)ws + ((size_t)x.rows * q.parts * 3 * sizeof(A) + 15) / 16 * 16);
+  return q;
+}
+
+template <class T, bool TOP, bool ENT, class Row>
+int launch_forward(Cut<T> q, Row row, const std::string& plan) {
+  void* args[] = {&q, &row};
+  const int64_t units = q.rows * q.parts;
+  int rc = launch_builtin((const void*)&vocab_read<T, TOP, Row, ENT>, plan, dim3(grid_of(ceil_div(units, kWaves))),
+                          dim3(64 * kWaves), args);
+  if (rc || q.parts == 1) return rc;
+  return launch_builtin((const void*)&vocab_join<T, TOP, Row, ENT>, plan + "|join", dim3(grid_of(q.rows)), dim3(64), args);
+}
+
+// The gradient's segments: blocks of 256 threads, at most kUnroll vectors to a thread, and fewer where that leaves
+// compute units without work.
+template <class T, class Row>
+int launch_grad(const Rows& x, double temperature, char* dx, Row row, const std::string& plan) {
+  typedef typename AccOf<T>::type A;
+  GradCut<T> q;
+  const int64_t vectors = ceil_div(x.cols, Width<T>::value);
+  q.x = (const T*)x.ptr;
+  q.xs = x.stride, q.rows = x.rows, q.cols = x.cols;
+  q.segs = (int)ceil_div(vectors, 256 * kUnroll);
+  if (x.rows * q.segs < 4 * compute_units())
+    q.segs = (int)std::max<int64_t>(q.segs, std::min<int64_t>(ceil_div(vectors, 256), ceil_div(4 * compute_units(), x.rows)));
+  q.per = ceil_div(vectors, q.segs);
+  q.c = (A)(kLog2E / temperature);
+  q.dx = (T*)dx;
+  void* args[] = {&q, &row};
+  return launch_builtin((const void*)&vocab_grad<T, Row>, plan, dim3(grid_of(x.rows * q.segs)), dim3(256), args);
+}
 
 template <class F>
 int by_type(int x, F&& f) {
@@ -354,7 +791,8 @@ int indices_of(const char* what, const char* name, const thx_array* a, const thx
 }
 
 int token_logprob(const thx_array* logits, const thx_array* tokens, double temperature, int n_top, const thx_array* log_prob,
-                  const thx_array* entropy, const thx_array* top, const thx_array* top_at, const thx_array* stats, int flags) {
+                  const thx_array* entropy, const thx_array* top, const thx_array* top_at, const thx_array* stats, void* ws,
+                  size_t ws_bytes, int flags) {
   const char* what = "token log probabilities";
   const bool dry = (flags & THX_DRY_RUN) != 0;
   Rows in[2], out[5];
@@ -374,18 +812,18 @@ int token_logprob(const thx_array* logits, const thx_array* tokens, double tempe
   for (int k = 0; k < 5; ++k)
     if ((rc = contiguous_rows(what, "a result", out[k]))) return rc;
   if ((rc = no_overlap(what, out, 5, in, 2)) && !dry) return rc;
-  const std::string plan = "lp|rows";
+  if ((rc = check_workspace(what, ws, ws_bytes, partial_bytes(in[0], n_top), flags))) return rc;
+  const std::string plan = plan_of("lp", in[0]) + (n_top ? "|top" : "");
   set_last_plan(plan);
   if (dry || !in[0].rows) return THX_OK;
   if ((rc = ensure_init())) return rc;
   return by_type(in[0].dtype, [&](auto t) {
     typedef decltype(t) T;
     typedef typename AccOf<T>::type A;
-    A c = (A)(kLog2E / temperature), inv_t = (A)(1.0 / temperature);
-    int t64 = in[1].dtype == THX_I64;
-    LpOut<A> o = {(A*)out[0].ptr, (A*)out[1].ptr, (A*)out[3].ptr, (int64_t*)out[4].ptr, (A*)out[2].ptr};
-    void* args[] = {&in[0].ptr, &in[0].stride, &in[0].rows, &in[0].cols, &in[1].ptr, &in[1].stride, &t64, &c, &inv_t, &n_top, &o};
-    return launch_builtin((const void*)&lp_forward<T>, plan, dim3(grid_of(in[0].rows)), dim3(256), args);
+    const LpRow<T> row = {in[1].ptr, in[1].stride, in[1].dtype == THX_I64, n_top, (A)(1.0 / temperature),
+                          {(A*)out[0].ptr, (A*)out[1].ptr, (A*)out[3].ptr, (int64_t*)out[4].ptr, (A*)out[2].ptr}};
+    const Cut<T> q = cut_of<T>(in[0], temperature, ws);
+    return n_top ? launch_forward<T, true, true>(q, row, plan) : launch_forward<T, false, true>(q, row, plan);
   });
 }
 
@@ -414,19 +852,17 @@ int token_logprob_grad(const thx_array* logits, const thx_array* tokens, const t
   if ((rc = like_rows(what, "dlogits", dx, logits, in[0].dtype, in[0].cols, flags, &out))) return rc;
   if ((rc = contiguous_rows(what, "dlogits", out))) return rc;
   if ((rc = no_overlap(what, &out, 1, in, 8)) && !dry) return rc;
-  const std::string plan = "lpg|rows";
+  const std::string plan = "lpg|t" + std::to_string(in[0].dtype);
   set_last_plan(plan);
   if (dry || !in[0].rows) return THX_OK;
   if ((rc = ensure_init())) return rc;
   return by_type(in[0].dtype, [&](auto t) {
     typedef decltype(t) T;
     typedef typename AccOf<T>::type A;
-    A c = (A)(kLog2E / temperature), inv_t = (A)(1.0 / temperature);
-    LpGrad<A> q = {in[1].ptr, in[1].stride, in[1].dtype == THX_I64, (const A*)in[2].ptr, in[2].stride, (const A*)in[3].ptr,
+    const LpGrad<A> q = {in[1].ptr, in[1].stride, in[1].dtype == THX_I64, (const A*)in[2].ptr, in[2].stride, (const A*)in[3].ptr,
                    in[3].stride, (const int64_t*)in[4].ptr, in[4].stride, (int)n_top, (const A*)in[5].ptr, in[5].stride,
-                   (const A*)in[6].ptr, in[6].stride, (const A*)in[7].ptr, in[7].stride};
-    void* args[] = {&in[0].ptr, &in[0].stride, &in[0].rows, &in[0].cols, &q, &c, &inv_t, &out.ptr};
-    return launch_builtin((const void*)&lp_backward<T>, plan, dim3(grid_of(in[0].rows)), dim3(256), args);
+                   (const A*)in[6].ptr, in[6].stride, (const A*)in[7].ptr, in[7].stride, (A)(1.0 / temperature)};
+    return launch_grad<T>(in[0], temperature, out.ptr, q, plan);
   });
 }
 
@@ -451,7 +887,7 @@ Teacher<A> teacher_args(const Rows& t, const Rows& ids) {
 }
 
 int topk_distill(const thx_array* logits, const thx_array* teacher, const thx_array* tokens, double temperature,
-                 const thx_array* loss, const thx_array* stats, int flags) {
+                 const thx_array* loss, const thx_array* stats, void* ws, size_t ws_bytes, int flags) {
   const char* what = "distillation loss";
   const bool dry = (flags & THX_DRY_RUN) != 0;
   Rows in[3], out[2];
@@ -464,17 +900,17 @@ int topk_distill(const thx_array* logits, const thx_array* teacher, const thx_ar
   for (int k = 0; k < 2; ++k)
     if ((rc = contiguous_rows(what, "a result", out[k]))) return rc;
   if ((rc = no_overlap(what, out, 2, in, 3)) && !dry) return rc;
-  const std::string plan = "kd|rows";
+  if ((rc = check_workspace(what, ws, ws_bytes, partial_bytes(in[0], 0), flags))) return rc;
+  const std::string plan = plan_of("kd", in[0]);
   set_last_plan(plan);
   if (dry || !in[0].rows) return THX_OK;
   if ((rc = ensure_init())) return rc;
   return by_type(in[0].dtype, [&](auto t) {
     typedef decltype(t) T;
     typedef typename AccOf<T>::type A;
-    A c = (A)(kLog2E / temperature), inv_t = (A)(1.0 / temperature), t2 = (A)(temperature * temperature);
-    Teacher<A> q = teacher_args<A>(in[1], in[2]);
-    void* args[] = {&in[0].ptr, &in[0].stride, &in[0].rows, &in[0].cols, &q, &c, &inv_t, &t2, &out[0].ptr, &out[1].ptr};
-    return launch_builtin((const void*)&kd_forward<T>, plan, dim3(grid_of(in[0].rows)), dim3(256), args);
+    const KdRow<T> row = {teacher_args<A>(in[1], in[2]), (A)(1.0 / temperature), (A)(temperature * temperature),
+                          (A*)out[0].ptr, (A*)out[1].ptr};
+    return launch_forward<T, false, false>(cut_of<T>(in[0], temperature, ws), row, plan);
   });
 }
 
@@ -492,19 +928,26 @@ int topk_distill_grad(const thx_array* logits, const thx_array* teacher, const t
   if ((rc = like_rows(what, "dlogits", dx, logits, in[0].dtype, in[0].cols, flags, &out))) return rc;
   if ((rc = contiguous_rows(what, "dlogits", out))) return rc;
   if ((rc = no_overlap(what, &out, 1, in, 5)) && !dry) return rc;
-  const std::string plan = "kdg|rows";
+  const std::string plan = "kdg|t" + std::to_string(in[0].dtype);
   set_last_plan(plan);
   if (dry || !in[0].rows) return THX_OK;
   if ((rc = ensure_init())) return rc;
   return by_type(in[0].dtype, [&](auto t) {
     typedef decltype(t) T;
     typedef typename AccOf<T>::type A;
-    A c = (A)(kLog2E / temperature), tt = (A)temperature;
-    Teacher<A> q = teacher_args<A>(in[1], in[2]);
-    void* args[] = {&in[0].ptr, &in[0].stride, &in[0].rows, &in[0].cols, &q, &in[3].ptr, &in[3].stride, &in[4].ptr,
-                    &in[4].stride, &c, &tt, &out.ptr};
-    return launch_builtin((const void*)&kd_backward<T>, plan, dim3(grid_of(in[0].rows)), dim3(256), args);
+    const KdGrad<A> row = {teacher_args<A>(in[1], in[2]), (const A*)in[3].ptr, in[3].stride, (const A*)in[4].ptr,
+                           in[4].stride, (A)(kLog2E / temperature), (A)temperature};
+    return launch_grad<T>(in[0], temperature, out.ptr, row, plan);
   });
+}
+
+int workspace_of(const char* what, const thx_array* logits, int n_top, size_t* nbytes) {
+  if (!logits || !nbytes) return fail(THX_ERR_ARG, "%s: null argument", what);
+  if (n_top < 0 || n_top > THX_MAX_TOP) return fail(THX_ERR_ARG, "%s: %d alternatives (at most %d)", what, n_top, THX_MAX_TOP);
+  Rows r;
+  int rc = logits_of(what, logits, 1.0, THX_DRY_RUN, &r);
+  if (!rc) *nbytes = partial_bytes(r, n_top);
+  return rc;
 }
 
 }  // namespace
@@ -516,9 +959,7 @@ extern "C" {
 
 int thx_token_logprob_workspace(const thx_array* logits, int n_top, size_t* nbytes) {
   return guarded("thx_token_logprob_workspace", [&] {
-    if (!logits || !nbytes) return fail(THX_ERR_ARG, "thx_token_logprob_workspace: null argument");
-    *nbytes = 0;
-    return (int)THX_OK;
+    return workspace_of("thx_token_logprob_workspace", logits, n_top, nbytes);
   });
 }
 
@@ -527,7 +968,8 @@ int thx_token_logprob_call(const thx_array* logits, const thx_array* tokens, dou
                            const thx_array* top_tokens, const thx_array* stats, void* workspace,
                            size_t workspace_bytes, int flags) {
   return guarded("thx_token_logprob_call", [&] {
-    return token_logprob(logits, tokens, temperature, n_top, log_prob, entropy, top_log_probs, top_tokens, stats, flags);
+    return token_logprob(logits, tokens, temperature, n_top, log_prob, entropy, top_log_probs, top_tokens, stats, workspace,
+                         workspace_bytes, flags);
   });
 }
 
@@ -543,9 +985,7 @@ int thx_token_logprob_grad_call(const thx_array* logits, const thx_array* tokens
 
 int thx_topk_distill_workspace(const thx_array* logits, size_t* nbytes) {
   return guarded("thx_topk_distill_workspace", [&] {
-    if (!logits || !nbytes) return fail(THX_ERR_ARG, "thx_topk_distill_workspace: null argument");
-    *nbytes = 0;
-    return (int)THX_OK;
+    return workspace_of("thx_topk_distill_workspace", logits, 0, nbytes);
   });
 }
 
@@ -553,7 +993,7 @@ int thx_topk_distill_call(const thx_array* logits, const thx_array* teacher, con
                           const thx_array* loss, const thx_array* stats, void* workspace, size_t workspace_bytes,
                           int flags) {
   return guarded("thx_topk_distill_call",
-                 [&] { return topk_distill(logits, teacher, tokens, temperature, loss, stats, flags); });
+                 [&] { return topk_distill(logits, teacher, tokens, temperature, loss, stats, workspace, workspace_bytes, flags); });
 }
 
 int thx_topk_distill_grad_call(const thx_array* logits, const thx_array* teacher, const thx_array* tokens,
