@@ -9,6 +9,260 @@ namespace {
 template <class T> struct AccOf { typedef float type; };
 template <> struct AccOf<double> { typedef double type; };
 
+// ---- rows held in registers ----------------------------------------------------------------------------------------
+//
+// TPR threads share a row, each holding VPT vectors of 16 bytes of it from the one time it is read: the mean, the squares
+// around the mean and the result come out of registers.  Up to 64 threads of one wave need nothing but shuffles; larger
+// groups are whole blocks and pass the sums of their waves through LDS.
+
+template <class T> struct Width { enum { value = 16 / (int)sizeof(T) }; };
+
+// Sums of N values over the TPR threads of a row, in every one of them.  `lds`: N * TPR / 64 values per call, two sets of
+// them used in turn, so that one barrier a call is enough: a set is written again two calls later, and by then every
+// wave has passed the barrier of the call between, behind its reads.
+template <int TPR, int N, class A>
+THX_DEV void row_sums(A (&v)[N], A* lds, int& turn) {
+#pragma unroll
+  for (int m = (TPR < 64 ? TPR : 64) / 2; m >= 1; m >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], m, 64);
+  if constexpr (TPR > 64) {
+    constexpr int W = TPR / 64;
+    A* set = lds + turn * N * W;
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < N; ++k) set[k * W + threadIdx.x / 64] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      v[k] = set[k * W];
+#pragma unroll
+      for (int w = 1; w < W; ++w) v[k] += set[k * W + w];
+    }
+  }
+}
+
+// Vector i of an array of `cols` elements; what lies behind the end is 0.
+template <class T, int V>
+THX_DEV void load_edge(Vec<T, V>& v, const T* p, int64_t i, int64_t cols) {
+  if ((i + 1) * V <= cols) {
+    load_vec<T, V, false, true>(v, p + i * V);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v.v[e] = i * V + e < cols ? p[i * V + e] : (T)0;
+  }
+}
+template <class T, int V>
+THX_DEV void store_edge(T* p, const Vec<T, V>& v, int64_t i, int64_t cols) {
+  if ((i + 1) * V <= cols) {
+    store_vec<T, V, false, true>(p + i * V, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (i * V + e < cols) p[i * V + e] = v.v[e];
+  }
+}
+
+THX_DEV float rsqrt_of(float v) { return 1.0f / sqrtf(v); }
+THX_DEV double rsqrt_of(double v) { return 1.0 / sqrt(v); }
+
+template <int TPR> struct Block { enum { threads = TPR > 256 ? TPR : 256, rows = threads / TPR }; };
+
+template <class T, class P, int TPR, int VPT>
+__global__ void __launch_bounds__(Block<TPR>::threads) ln_forward(const T* x, int64_t xs, int64_t rows, int64_t cols,
+                                                                  const P* gamma, const P* beta, double eps, T* y,
+                                                                  typename AccOf<T>::type* mean,
+                                                                  typename AccOf<T>::type* invstd) {
+  typedef typename AccOf<T>::type A;
+  constexpr int V = Width<T>::value, RPB = Block<TPR>::rows;
+  __shared__ A lds[TPR > 64 ? 2 * TPR / 64 : 1];
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  const A n = (A)cols;
+  int turn = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t r = r0 + group < rows ? r0 + group : rows - 1;  // threads without a row repeat the last one
+    const T* xr = x + r * xs;
+    Vec<T, V> v[VPT];
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) load_edge(v[u], xr, u * TPR + t, cols);
+    A sum[1] = {0};
+#pragma unroll
+    for (int u = 0; u < VPT; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[0] += (A)v[u].v[e];
+    row_sums<TPR>(sum, lds, turn);
+    const A mu = sum[0] / n;
+    A sq[1] = {0};
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      const int64_t left = cols - (int64_t)(u * TPR + t) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const A d = (A)v[u].v[e] - mu;
+        sq[0] += e < left ? d * d : (A)0;
+      }
+    }
+    row_sums<TPR>(sq, lds, turn);
+    const A inv = rsqrt_of(sq[0] / n + (A)eps);
+    T* yr = y + r * cols;
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      const int64_t i = u * TPR + t;
+      if (i * V >= cols) continue;
+      Vec<P, V> g, b;
+      if (gamma) load_edge(g, gamma, i, cols);
+      if (beta) load_edge(b, beta, i, cols);
+      Vec<T, V> o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        A w = ((A)v[u].v[e] - mu) * inv;
+        if (gamma) w *= (A)g.v[e];
+        if (beta) w += (A)b.v[e];
+        o.v[e] = (T)w;
+      }
+      store_edge(yr, o, i, cols);
+    }
+    if (t == 0) mean[r] = mu, invstd[r] = inv;
+  }
+}
+
+// The gradients.  A block goes through rows blockIdx.x, + gridDim.x, ... (RPB of them at a time) and keeps the sums of
+// dy * xhat and dy of its rows in registers, per column; at the end it leaves them in partial[block][2][cols], which
+// ln_join adds up.  One pass over x and dy serves all three gradients.
+template <class T, class P, int TPR, int VPT, bool PARAMS>
+__global__ void __launch_bounds__(Block<TPR>::threads) ln_backward(const T* x, int64_t xs, const T* dy, int64_t ds,
+                                                                   int64_t rows, int64_t cols, const P* gamma,
+                                                                   const typename AccOf<T>::type* mean, int64_t ms,
+                                                                   const typename AccOf<T>::type* invstd, int64_t is, T* dx,
+                                                                   typename AccOf<T>::type* partial) {
+  typedef typename AccOf<T>::type A;
+  constexpr int V = Width<T>::value, RPB = Block<TPR>::rows;
+  __shared__ A lds[TPR > 64 ? 4 * TPR / 64 : 1];
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  const A n = (A)cols;
+  int turn = 0;
+  A dg[PARAMS ? VPT : 1][V], db[PARAMS ? VPT : 1][V];
+#pragma unroll
+  for (int u = 0; u < (PARAMS ? VPT : 1); ++u)
+#pragma unroll
+    for (int e = 0; e < V; ++e) dg[u][e] = db[u][e] = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    const bool live = r0 + group < rows;
+    const int64_t r = live ? r0 + group : rows - 1;
+    const T *xr = x + r * xs, *dr = dy + r * ds;
+    Vec<T, V> v[VPT], d[VPT];
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      load_edge(v[u], xr, u * TPR + t, cols);
+      load_edge(d[u], dr, u * TPR + t, cols);  // 0 behind the end: those columns add nothing
+    }
+    const A mu = mean[r * ms], inv = invstd[r * is];
+    A s[2] = {0, 0};
+    Vec<P, V> g[VPT];
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      if (gamma) load_edge(g[u], gamma, u * TPR + t, cols);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const A dv = (A)d[u].v[e], a = gamma ? dv * (A)g[u].v[e] : dv, xh = ((A)v[u].v[e] - mu) * inv;
+        s[0] += a;
+        s[1] += a * xh;
+        if (PARAMS && live) {
+          dg[u][e] += dv * xh;
+          db[u][e] += dv;
+        }
+      }
+    }
+    row_sums<TPR>(s, lds, turn);
+    s[0] /= n;
+    s[1] /= n;
+    T* out = dx + r * cols;
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      const int64_t i = u * TPR + t;
+      if (i * V >= cols) continue;
+      Vec<T, V> o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const A dv = (A)d[u].v[e], a = gamma ? dv * (A)g[u].v[e] : dv, xh = ((A)v[u].v[e] - mu) * inv;
+        o.v[e] = (T)(inv * (a - s[0] - xh * s[1]));
+      }
+      store_edge(out, o, i, cols);
+    }
+  }
+  if constexpr (PARAMS) {
+    // the groups of a block first, through LDS, one column vector at a time
+    constexpr int VEC = V * 2;
+    __shared__ A fold[RPB > 1 ? RPB * TPR * VEC : 1];
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      if constexpr (RPB > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          fold[(2 * e) * RPB * TPR + threadIdx.x] = dg[u][e];
+          fold[(2 * e + 1) * RPB * TPR + threadIdx.x] = db[u][e];
+        }
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            for (int k = 1; k < RPB; ++k) {
+              dg[u][e] += fold[(2 * e) * RPB * TPR + k * TPR + t];
+              db[u][e] += fold[(2 * e + 1) * RPB * TPR + k * TPR + t];
+            }
+        }
+      }
+      if (group == 0) {
+        A* to = partial + (int64_t)blockIdx.x * 2 * cols;
+        const int64_t j = (int64_t)(u * TPR + t) * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (j + e < cols) {
+            to[j + e] = dg[u][e];
+            to[cols + j + e] = db[u][e];
+          }
+      }
+    }
+  }
+}
+
+// Adds up the blocks' sums: 64 columns by 16 slices of the blocks to a block here, blockIdx.y 0 for gamma, 1 for beta.
+template <class A, class P>
+__global__ void __launch_bounds__(1024) ln_join(const A* partial, int blocks, int64_t cols, P* dgamma, P* dbeta) {
+  __shared__ A lds[16][64];
+  const int lane = threadIdx.x & 63, slice = threadIdx.x / 64;
+  P* to = blockIdx.y ? dbeta : dgamma;
+  const A* from = partial + (blockIdx.y ? cols : 0);
+  for (int64_t c0 = (int64_t)blockIdx.x * 64; c0 < cols; c0 += (int64_t)gridDim.x * 64) {
+    const int64_t c = c0 + lane;
+    A s = 0;
+    if (c < cols) {
+      int k = slice;
+      for (; k + 48 < blocks; k += 64) {
+        const A p0 = from[(int64_t)k * 2 * cols + c], p1 = from[(int64_t)(k + 16) * 2 * cols + c];
+        const A p2 = from[(int64_t)(k + 32) * 2 * cols + c], p3 = from[(int64_t)(k + 48) * 2 * cols + c];
+        s += (p0 + p1) + (p2 + p3);
+      }
+      for (; k < blocks; k += 16) s += from[(int64_t)k * 2 * cols + c];
+    }
+    lds[slice][lane] = s;
+    __syncthreads();
+    if (slice == 0 && c < cols) {
+#pragma unroll
+      for (int k = 1; k < 16; ++k) s += lds[k][lane];
+      to[c] = (P)s;
+    }
+    __syncthreads();
+  }
+}
+
+// ---- any row -------------------------------------------------------------------------------------------------------
+//
+// Rows beyond what a block of 1024 threads holds, and parameters that do not lie side by side: one block per row, read
+// once per step (the later reads come from the caches), and the parameters' sums by columns in a pass of their own.
+
 template <class A>
 THX_DEV A block_sum(A v, A* lds) {
 #pragma unroll
@@ -22,11 +276,11 @@ THX_DEV A block_sum(A v, A* lds) {
 }
 
 template <class T, class P>
-__global__ void __launch_bounds__(256) ln_forward(const T* x, int64_t xs, int64_t rows, int64_t cols, const P* gamma, int64_t gs,
+__global__ void __launch_bounds__(1024) ln_forward_any(const T* x, int64_t xs, int64_t rows, int64_t cols, const P* gamma, int64_t gs,
                                                   const P* beta, int64_t bs, double eps, T* y,
                                                   typename AccOf<T>::type* mean, typename AccOf<T>::type* invstd) {
   typedef typename AccOf<T>::type A;
-  __shared__ A lds[4];
+  __shared__ A lds[16];
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xr = x + r * xs;
     A s = 0;
@@ -49,11 +303,11 @@ __global__ void __launch_bounds__(256) ln_forward(const T* x, int64_t xs, int64_
 }
 
 template <class T, class P>
-__global__ void __launch_bounds__(256) ln_grad_rows(const T* x, int64_t xs, const T* dy, int64_t ds, int64_t rows, int64_t cols,
+__global__ void __launch_bounds__(1024) ln_backward_any(const T* x, int64_t xs, const T* dy, int64_t ds, int64_t rows, int64_t cols,
                                                     const P* gamma, int64_t gs, const typename AccOf<T>::type* mean,
                                                     int64_t ms, const typename AccOf<T>::type* invstd, int64_t is, T* dx) {
   typedef typename AccOf<T>::type A;
-  __shared__ A lds[4];
+  __shared__ A lds[16];
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T *xr = x + r * xs, *dr = dy + r * ds;
     const A mu = mean[r * ms], inv = invstd[r * is];
@@ -74,7 +328,7 @@ __global__ void __launch_bounds__(256) ln_grad_rows(const T* x, int64_t xs, cons
 
 // Sums over a slice of the rows, one column per thread: partial[slice][2][cols].
 template <class T>
-__global__ void __launch_bounds__(256) ln_grad_params(const T* x, int64_t xs, const T* dy, int64_t ds, int64_t rows,
+__global__ void __launch_bounds__(1024) ln_params_any(const T* x, int64_t xs, const T* dy, int64_t ds, int64_t rows,
                                                       int64_t cols, const typename AccOf<T>::type* mean, int64_t ms,
                                                       const typename AccOf<T>::type* invstd, int64_t is,
                                                       typename AccOf<T>::type* partial) {
@@ -90,19 +344,6 @@ __global__ void __launch_bounds__(256) ln_grad_params(const T* x, int64_t xs, co
     }
     partial[(int64_t)blockIdx.y * 2 * cols + c] = g;
     partial[((int64_t)blockIdx.y * 2 + 1) * cols + c] = b;
-  }
-}
-
-template <class A, class P>
-__global__ void __launch_bounds__(256) ln_grad_join(const A* partial, int slices, int64_t cols, P* dgamma, P* dbeta) {
-  for (int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; c < cols; c += (int64_t)gridDim.x * blockDim.x) {
-    A g = 0, b = 0;
-    for (int s = 0; s < slices; ++s) {
-      g += partial[(int64_t)s * 2 * cols + c];
-      b += partial[((int64_t)s * 2 + 1) * cols + c];
-    }
-    if (dgamma) dgamma[c] = (P)g;
-    if (dbeta) dbeta[c] = (P)b;
   }
 }
 
@@ -127,7 +368,76 @@ int param_of(const char* what, const char* name, const thx_array* a, int dtype, 
 
 unsigned grid_of(int64_t n) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(n, 1 << 20)); }
 
+// How a call's rows are laid out over threads; tpr 0: the kernels for any row.
+struct Shape {
+  int tpr = 0, vpt = 0;
+};
+
+// The smallest group of threads that holds a row in registers.  Forward: up to 8 vectors to a thread, so that rows of up to
+// 4096 halves stay within one wave and need no barrier.  Backward a thread keeps two more sums per column, so a quarter of
+// the columns, and longer rows take whole blocks.
+Shape shape_of(int64_t cols, int dtype, bool backward, bool packed) {
+  const int64_t nv = (cols * dtype_size(dtype) + 15) / 16;
+  static const Shape forward[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {64, 8}, {256, 4}, {256, 8}, {1024, 8}};
+  static const Shape back[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {1024, 1}, {1024, 2}};
+  Shape none;
+  if (!packed || !cols) return none;
+  if (backward) {
+    for (const Shape& s : back)
+      if (nv <= (int64_t)s.tpr * s.vpt) return s;
+  } else {
+    for (const Shape& s : forward)
+      if (nv <= (int64_t)s.tpr * s.vpt) return s;
+  }
+  return none;
+}
+
+// Blocks of the gradients' pass: as many as the device runs at once, no more than there are rows for.  Each leaves one
+// set of sums, so more of them would only be more to add up.
+int64_t backward_blocks(const Shape& s, int64_t rows) {
+  const int64_t per = s.tpr > 256 ? 1 : 256 / s.tpr;
+  const int64_t most = (int64_t)compute_units() * (s.tpr > 256 ? 1 : 4);
+  return std::max<int64_t>(1, std::min<int64_t>(most, (rows + per - 1) / per));
+}
+
 int slices_of(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>(64, rows / 64)); }
+
+// f(integral constants TPR, VPT) for a shape.
+template <int TPR, int VPT> struct Held { enum { tpr = TPR, vpt = VPT }; };
+template <class F>
+int by_shape(const Shape& s, F&& f) {
+  switch (s.tpr * 16 + s.vpt) {
+    case 8 * 16 + 1: return f(Held<8, 1>());
+    case 16 * 16 + 1: return f(Held<16, 1>());
+    case 32 * 16 + 1: return f(Held<32, 1>());
+    case 64 * 16 + 1: return f(Held<64, 1>());
+    case 64 * 16 + 2: return f(Held<64, 2>());
+    case 64 * 16 + 4: return f(Held<64, 4>());
+    case 64 * 16 + 8: return f(Held<64, 8>());
+    case 256 * 16 + 4: return f(Held<256, 4>());
+    case 256 * 16 + 8: return f(Held<256, 8>());
+    default: return f(Held<1024, 8>());
+  }
+}
+template <class F>
+int by_back_shape(const Shape& s, F&& f) {
+  switch (s.tpr * 16 + s.vpt) {
+    case 8 * 16 + 1: return f(Held<8, 1>());
+    case 16 * 16 + 1: return f(Held<16, 1>());
+    case 32 * 16 + 1: return f(Held<32, 1>());
+    case 64 * 16 + 1: return f(Held<64, 1>());
+    case 64 * 16 + 2: return f(Held<64, 2>());
+    case 256 * 16 + 1: return f(Held<256, 1>());
+    case 256 * 16 + 2: return f(Held<256, 2>());
+    case 1024 * 16 + 1: return f(Held<1024, 1>());
+    default: return f(Held<1024, 2>());
+  }
+}
+
+std::string plan_of(const char* name, int dtype, const Shape& s) {
+  return std::string(name) + "|t" + std::to_string(dtype) +
+         (s.tpr ? "|r" + std::to_string(s.tpr) + "x" + std::to_string(s.vpt) : std::string("|any"));
+}
 
 // f(T(), P()) for the element types of the rows and of the parameters.
 template <class F>
@@ -156,17 +466,35 @@ int layernorm(const thx_array* x, const thx_array* gamma, const thx_array* beta,
   for (int k = 0; k < 3; ++k)
     if ((rc = contiguous_rows(what, "a result", out[k]))) return rc;
   if ((rc = no_overlap(what, out, 3, in, 3)) && !dry) return rc;
-  const std::string plan = "ln|rows";
+  const bool packed = (!gamma || in[0].cols <= 1 || in[1].stride == 1) && (!beta || in[0].cols <= 1 || in[2].stride == 1);
+  const Shape shape = shape_of(in[0].cols, in[0].dtype, false, packed);
+  const std::string plan = plan_of("ln", in[0].dtype, shape);
   set_last_plan(plan);
   if (dry || !in[0].rows) return THX_OK;
   if ((rc = ensure_init())) return rc;
   return by_types(in[0].dtype, pt, [&](auto t, auto p) {
     typedef decltype(t) T;
     typedef decltype(p) P;
-    void* args[] = {&in[0].ptr, &in[0].stride, &in[0].rows, &in[0].cols, &in[1].ptr, &in[1].stride, &in[2].ptr,
-                    &in[2].stride, &epsilon, &out[0].ptr, &out[1].ptr, &out[2].ptr};
-    return launch_builtin((const void*)&ln_forward<T, P>, plan, dim3(grid_of(in[0].rows)), dim3(256), args);
+    if (!shape.tpr) {
+      void* args[] = {&in[0].ptr, &in[0].stride, &in[0].rows, &in[0].cols, &in[1].ptr, &in[1].stride, &in[2].ptr,
+                      &in[2].stride, &epsilon, &out[0].ptr, &out[1].ptr, &out[2].ptr};
+      return launch_builtin((const void*)&ln_forward_any<T, P>, plan, dim3(grid_of(in[0].rows)), dim3(1024), args);
+    }
+    return by_shape(shape, [&](auto h) {
+      constexpr int TPR = decltype(h)::tpr, VPT = decltype(h)::vpt;
+      void* args[] = {&in[0].ptr, &in[0].stride, &in[0].rows, &in[0].cols, &in[1].ptr, &in[2].ptr, &epsilon, &out[0].ptr,
+                      &out[1].ptr, &out[2].ptr};
+      const int64_t per = Block<TPR>::rows;
+      return launch_builtin((const void*)&ln_forward<T, P, TPR, VPT>, plan, dim3(grid_of((in[0].rows + per - 1) / per)),
+                            dim3(Block<TPR>::threads), args);
+    });
   });
+}
+
+// Blocks that leave sums of the parameters' gradients, for either family of kernels.
+int64_t partial_blocks(const Rows& x, bool packed) {
+  const Shape s = shape_of(x.cols, x.dtype, true, packed);
+  return s.tpr ? backward_blocks(s, x.rows) : slices_of(x.rows);
 }
 
 int layernorm_grad_bytes(const thx_array* x, const thx_array* dgamma, size_t* nbytes) {
@@ -174,7 +502,9 @@ int layernorm_grad_bytes(const thx_array* x, const thx_array* dgamma, size_t* nb
   Rows r;
   int rc = rows_of("layer normalization gradient", "x", x, -1, 1, THX_DRY_RUN, &r);
   if (rc) return rc;
-  *nbytes = dgamma ? (size_t)slices_of(r.rows) * 2 * r.cols * dtype_size(acc_code(r.dtype)) : 0;
+  // whichever gamma's stride asks for
+  const int64_t blocks = std::max(partial_blocks(r, true), partial_blocks(r, false));
+  *nbytes = dgamma ? (size_t)blocks * 2 * r.cols * dtype_size(acc_code(r.dtype)) : 0;
   return THX_OK;
 }
 
@@ -204,29 +534,44 @@ int layernorm_grad(const thx_array* x, const thx_array* dy, const thx_array* gam
   size_t need = 0;
   if ((rc = layernorm_grad_bytes(x, dgamma, &need))) return rc;
   if ((rc = check_workspace(what, ws, ws_bytes, need, flags))) return rc;
-  const std::string plan = "lng|rows";
+  const bool packed = !gamma || in[0].cols <= 1 || in[4].stride == 1;
+  const Shape shape = shape_of(in[0].cols, in[0].dtype, true, packed);
+  const std::string plan = plan_of("lng", in[0].dtype, shape);
   set_last_plan(plan);
-  if (dry) return THX_OK;
+  if (dry || !in[0].cols) return THX_OK;
   if ((rc = ensure_init())) return rc;
   return by_types(in[0].dtype, pt, [&](auto t, auto p) {
     typedef decltype(t) T;
     typedef decltype(p) P;
     typedef typename AccOf<T>::type A;
     int rc = THX_OK;
-    if (in[0].rows && in[0].cols) {
-      void* args[] = {&in[0].ptr, &in[0].stride, &in[1].ptr, &in[1].stride, &in[0].rows, &in[0].cols, &in[4].ptr,
-                      &in[4].stride, &in[2].ptr, &in[2].stride, &in[3].ptr, &in[3].stride, &out[0].ptr};
-      rc = launch_builtin((const void*)&ln_grad_rows<T, P>, plan, dim3(grid_of(in[0].rows)), dim3(256), args);
+    int blocks = (int)partial_blocks(in[0], packed);
+    const unsigned columns = grid_of((in[0].cols + 63) / 64);
+    if (shape.tpr) {
+      rc = by_back_shape(shape, [&](auto h) {
+        constexpr int TPR = decltype(h)::tpr, VPT = decltype(h)::vpt;
+        void* args[] = {&in[0].ptr, &in[0].stride, &in[1].ptr, &in[1].stride, &in[0].rows, &in[0].cols, &in[4].ptr,
+                        &in[2].ptr, &in[2].stride, &in[3].ptr, &in[3].stride, &out[0].ptr, &ws};
+        const void* kernel = dgamma ? (const void*)&ln_backward<T, P, TPR, VPT, true>
+                                    : (const void*)&ln_backward<T, P, TPR, VPT, false>;
+        return launch_builtin(kernel, plan, dim3(blocks), dim3(Block<TPR>::threads), args);
+      });
+    } else {
+      if (in[0].rows) {
+        void* args[] = {&in[0].ptr, &in[0].stride, &in[1].ptr, &in[1].stride, &in[0].rows, &in[0].cols, &in[4].ptr,
+                        &in[4].stride, &in[2].ptr, &in[2].stride, &in[3].ptr, &in[3].stride, &out[0].ptr};
+        rc = launch_builtin((const void*)&ln_backward_any<T, P>, plan, dim3(grid_of(in[0].rows)), dim3(1024), args);
+      }
+      if (!rc && dgamma) {
+        void* args[] = {&in[0].ptr, &in[0].stride, &in[1].ptr, &in[1].stride, &in[0].rows, &in[0].cols, &in[2].ptr,
+                        &in[2].stride, &in[3].ptr, &in[3].stride, &ws};
+        rc = launch_builtin((const void*)&ln_params_any<T>, plan, dim3(grid_of((in[0].cols + 255) / 256), blocks), dim3(256),
+                            args);
+      }
     }
-    if (rc || !dgamma || !in[0].cols) return rc;
-    int slices = slices_of(in[0].rows);
-    const unsigned blocks = grid_of((in[0].cols + 255) / 256);
-    void* args[] = {&in[0].ptr, &in[0].stride, &in[1].ptr, &in[1].stride, &in[0].rows, &in[0].cols, &in[2].ptr,
-                    &in[2].stride, &in[3].ptr, &in[3].stride, &ws};
-    rc = launch_builtin((const void*)&ln_grad_params<T>, plan, dim3(blocks, slices), dim3(256), args);
-    if (rc) return rc;
-    void* join[] = {&ws, &slices, &in[0].cols, &out[1].ptr, &out[2].ptr};
-    return launch_builtin((const void*)&ln_grad_join<A, P>, plan, dim3(blocks), dim3(256), join);
+    if (rc || !dgamma) return rc;
+    void* join[] = {&ws, &blocks, &in[0].cols, &out[1].ptr, &out[2].ptr};
+    return launch_builtin((const void*)&ln_join<A, P>, plan + "|join", dim3(columns, dbeta ? 2 : 1), dim3(1024), join);
   });
 }
 
