@@ -307,6 +307,19 @@ int thx_topk_distill_grad_call(const thx_array* logits, const thx_array* teacher
                                const thx_array* stats, const thx_array* g_loss, double temperature,
                                const thx_array* dlogits, int flags);
 
+/* A forward call and its gradient call in one, for gradients that are known beforehand (the weight of a loss): the row is
+ * read once.  Operands and results as in the two calls, without alternatives; the workspace is that of the forward
+ * call with n_top 0.  g_log_prob, g_entropy and g_loss are one value per row or, with every extent 1, one value for all
+ * rows (in the separate gradient calls as well). */
+int thx_token_logprob_train_call(const thx_array* logits, const thx_array* tokens, const thx_array* g_log_prob,
+                                 const thx_array* g_entropy, double temperature, const thx_array* log_prob,
+                                 const thx_array* entropy, const thx_array* stats, const thx_array* dlogits,
+                                 void* workspace, size_t workspace_bytes, int flags);
+int thx_topk_distill_train_call(const thx_array* logits, const thx_array* teacher, const thx_array* tokens,
+                                const thx_array* g_loss, double temperature, const thx_array* loss,
+                                const thx_array* stats, const thx_array* dlogits, void* workspace,
+                                size_t workspace_bytes, int flags);
+
 /* ---- inspection and timing ------------------------------------------------ */
 
 /* Name of the kernel plan used by the last elemwise / reduce call on this

@@ -188,8 +188,9 @@ def ln_function(dtype, pdtype, nd, n_params, eps, train):
     return _cache[key]
 
 
-def lp_function(dtype, idt, nd, n_top, temperature, given):
-    key = ("lp", dtype, idt, nd, n_top, temperature, given)
+def lp_function(dtype, idt, nd, n_top, temperature, given, fuse=True):
+    """``fuse``: the forward pass and the gradient in one launch (without alternatives), else two."""
+    key = ("lp", dtype, idt, nd, n_top, temperature, given, fuse)
     if key not in _cache:
         acc = acc_of(dtype)
         x, t = tensor(dtype, nd), tensor(idt, nd - 1)
@@ -199,18 +200,18 @@ def lp_function(dtype, idt, nd, n_top, temperature, given):
         ins = [x, t] + [cot[k] for k in range(3) if given[k]]
         if known:
             outs.append(th.grad(None, x, known_grads=known))
-        _cache[key] = th.function(ins, [Out(o, device=True) for o in outs])
+        _cache[key] = th.function(ins, [Out(o, device=True) for o in outs], fuse=fuse)
     return _cache[key]
 
 
-def kd_function(dtype, tdt, idt, nd, temperature, train):
-    key = ("kd", dtype, tdt, idt, nd, temperature, train)
+def kd_function(dtype, tdt, idt, nd, temperature, train, fuse=True):
+    key = ("kd", dtype, tdt, idt, nd, temperature, train, fuse)
     if key not in _cache:
         x, t, ids = tensor(dtype, nd), tensor(tdt, nd), tensor(idt, nd)
         g = tensor(acc_of(dtype), nd - 1)
         loss = T.nnet.topk_distillation_loss(x, t, ids, temperature=temperature)
         outs = [loss] + ([th.grad(None, x, known_grads={loss: g})] if train else [])
-        _cache[key] = th.function([x, t, ids] + ([g] if train else []), [Out(o, device=True) for o in outs])
+        _cache[key] = th.function([x, t, ids] + ([g] if train else []), [Out(o, device=True) for o in outs], fuse=fuse)
     return _cache[key]
 
 
@@ -235,12 +236,18 @@ def check_ln(x, gamma, beta, dy=None, eps=1e-5, dev=None, what=""):
 
 def check_lp(x, tokens, temperature=1.0, n_top=0, w=None, u=None, c=None, dev=None, what=""):
     given = tuple(v is not None for v in (w, u, c))
-    f = lp_function(str(x.dtype), str(tokens.dtype), x.ndim, n_top, temperature, given)
-    args = [x, tokens] + [v for v in (w, u, c) if v is not None]
+    ref = lp_ref(x, tokens, temperature, n_top, w, u, c)
+    for fuse in ([True, False] if any(given) and not n_top else [False]):
+        check_lp_call(x, tokens, temperature, n_top, given, [v for v in (w, u, c) if v is not None], dev, ref, fuse, what)
+
+
+def check_lp_call(x, tokens, temperature, n_top, given, cotangents, dev, ref, fuse, what):
+    f = lp_function(str(x.dtype), str(tokens.dtype), x.ndim, n_top, temperature, given, fuse)
+    assert any(type(n.op).__name__ == "HipTokenLogProbsTrain" for n in f.toposort()) == fuse
+    args = [x, tokens] + cotangents
     for k, v in (dev or {}).items():
         args[k] = v
     got = [o.to_numpy() for o in f(*args)]
-    ref = lp_ref(x, tokens, temperature, n_top, w, u, c)
     acc, n = acc_of(str(x.dtype)), chain(x.shape[-1])
     close(got[0], *ref["log_prob"], n, what + " log_prob", acc)
     close(got[1], *ref["entropy"], n, what + " entropy", acc)
@@ -255,12 +262,18 @@ def check_lp(x, tokens, temperature=1.0, n_top=0, w=None, u=None, c=None, dev=No
 
 
 def check_kd(x, teacher, ids, temperature=1.0, g=None, dev=None, what=""):
-    f = kd_function(str(x.dtype), str(teacher.dtype), str(ids.dtype), x.ndim, temperature, g is not None)
+    ref = kd_ref(x, teacher, ids, temperature, g)
+    for fuse in ([True, False] if g is not None else [False]):
+        check_kd_call(x, teacher, ids, temperature, g, dev, ref, fuse, what)
+
+
+def check_kd_call(x, teacher, ids, temperature, g, dev, ref, fuse, what):
+    f = kd_function(str(x.dtype), str(teacher.dtype), str(ids.dtype), x.ndim, temperature, g is not None, fuse)
+    assert any(type(n.op).__name__ == "HipTopKDistillationTrain" for n in f.toposort()) == fuse
     args = [x, teacher, ids] + ([g] if g is not None else [])
     for k, v in (dev or {}).items():
         args[k] = v
     got = [o.to_numpy() for o in f(*args)]
-    ref = kd_ref(x, teacher, ids, temperature, g)
     acc, n = acc_of(str(x.dtype)), chain(x.shape[-1]) + ids.shape[-1]
     assert got[0].dtype == np.dtype(acc)
     close(got[0], *ref["loss"], n, what + " loss", acc)
@@ -390,6 +403,7 @@ def test_layouts_of_the_operands(dtype):
         c = rng.standard_normal(lead + (4,)).astype(acc)
         for name, xd in layouts(x, rng):
             check_lp(x, tokens, n_top=4, w=w, u=u, c=c, dev={0: xd}, what="lp " + name)
+            check_lp(x, tokens, w=w, u=u, dev={0: xd}, what="lp " + name)
         teacher, ids = rng.standard_normal(lead + (5,)).astype("float32"), rng.integers(0, shape[-1], lead + (5,)).astype("int32")
         for (name, xd), (_, td), (_, idd) in zip(layouts(x, rng), reversed(list(layouts(teacher, rng))), layouts(ids, rng)):
             check_kd(x, teacher, ids, g=w, dev={0: xd, 1: td, 2: idd}, what="kd " + name)
@@ -409,7 +423,8 @@ def test_one_row_for_all():
 
 # ---- log probabilities -------------------------------------------------------------------------------------
 
-LP_SHAPES = [(1, 1), (1, 2), (2, 7), (3, 64), (5, 65), (1, 513), (4, 1000), (2, 3, 257), (300, 100), (17, 4097), (1, 16384),
+# held by one block of every size (up to 256 to 20480 vectors of 16 bytes), and beyond
+LP_SHAPES = [(3, 9000), (2, 20000), (3, 70000), (2, 150000), (2, 170001), (1, 1), (1, 2), (2, 7), (3, 64), (5, 65), (1, 513), (4, 1000), (2, 3, 257), (300, 100), (17, 4097), (1, 16384),
              (3, 32000), (1, 50257), (2, 131072), (700, 515), (70, 9001)]
 
 
@@ -426,6 +441,7 @@ def test_token_log_probs(shape, dtype):
     k = min(V, 20)
     check_lp(x, tokens, n_top=k, u=u, what="entropy alone")
     check_lp(x, tokens, temperature=2.0, n_top=k, w=w, u=u, c=rng.standard_normal(lead + (k,)).astype(acc), what="all")
+    check_lp(x, tokens, temperature=1.5, w=w, u=u, what="both gradients")
     check_lp(x, tokens, n_top=min(V, 64), what="most")
 
 
@@ -468,6 +484,7 @@ def test_masked_logits(dtype):
             x[4, :] = lowest
             x[4, ::3] = -INF
             check_lp(x, tokens, n_top=7, w=w, u=u, c=c, what="%s %s" % (shape, mask))
+            check_lp(x, tokens, w=w, u=u, what="%s %s" % (shape, mask))
             check_kd(x, teacher, ids, g=w, temperature=1.5, what="%s %s" % (shape, mask))
 
 
@@ -487,6 +504,7 @@ def test_nan_and_infinity_among_the_logits(dtype):
         tokens = rng.integers(0, shape[1], lead)
         w, u = [rng.standard_normal(lead).astype(acc) for _ in range(2)]
         check_lp(x, tokens, n_top=9, w=w, u=u, what=str(shape))
+        check_lp(x, tokens, w=w, u=u, what=str(shape))
         check_kd(x, rng.standard_normal(lead + (6,)).astype("float32"), rng.integers(0, shape[1], lead + (6,)), g=w,
                  what=str(shape))
 
@@ -498,6 +516,7 @@ def test_tokens_that_are_none_or_beyond_the_last_column():
     for idt in ("int32", "int64"):
         tokens = np.array([5, -1, 2999, 3000, -100, np.iinfo(idt).max], idt)
         check_lp(x, tokens, n_top=3, w=w, u=u, what=idt)
+        check_lp(x, tokens, w=w, u=u, what=idt)
         check_lp(x, tokens, u=u, what=idt + " entropy alone")     # the row's gradient does not go through the token
         ids = np.tile(np.array([5, 7, -1, 9, -3], idt), (6, 1))
         ids[1] = -1
@@ -515,6 +534,7 @@ def test_large_logits_keep_their_digits():
         x = (at + 8 * rng.standard_normal((4, 2000))).astype(dtype)
         w, u = [rng.standard_normal(4).astype(acc_of(dtype)) for _ in range(2)]
         check_lp(x, rng.integers(0, 2000, 4), n_top=5, w=w, u=u, what="%s %g" % (dtype, at))
+        check_lp(x, rng.integers(0, 2000, 4), w=w, u=u, what="%s %g" % (dtype, at))
         check_kd(x, rng.standard_normal((4, 6)).astype("float32"), rng.integers(0, 2000, (4, 6)), g=w, what="%s %g" % (dtype, at))
     x = logits(rng, (3, 700), "float16")
     for t in (1e-3, 50.0):
@@ -526,6 +546,7 @@ def test_no_rows():
         acc = acc_of(dtype)
         z = np.zeros((0,), acc)
         check_lp(np.zeros((0, 50), dtype), np.zeros((0,), "int64"), n_top=3, w=z, u=z, c=np.zeros((0, 3), acc))
+        check_lp(np.zeros((0, 50), dtype), np.zeros((0,), "int64"), w=z, u=z)
         check_kd(np.zeros((0, 50), dtype), np.zeros((0, 4), "float32"), np.zeros((0, 4), "int64"), g=z)
 
 
@@ -588,6 +609,24 @@ def test_gradients_are_those_of_differences():
         f = th.function(ins, cost, on_unused_input="ignore")
         g = th.function(ins, th.grad(cost, x), on_unused_input="ignore")(*vals)
         np.testing.assert_allclose(g, differences(f, vals, 0, 1e-6), rtol=1e-6, atol=1e-7)
+
+
+def test_one_weight_for_all_rows():
+    """The weight of a mean is read as one value, in one launch and in two."""
+    rng = np.random.default_rng(28)
+    x, t, teacher, ids = tensor("float16", 2), T.lvector(), T.fmatrix(), T.imatrix()
+    lp, h = T.nnet.token_log_probs(x, t)
+    kd = T.nnet.topk_distillation_loss(x, teacher, ids)
+    cost = T.mean(np.float32(64) * kd) - T.mean(lp)
+    vals = [logits(rng, (11, 777), "float16"), rng.integers(0, 777, 11), rng.standard_normal((11, 5)).astype("float32"),
+            rng.integers(0, 777, (11, 5)).astype("int32")]
+    one = np.ones(11)
+    a, b = lp_ref(vals[0], vals[1], w=-one / 11), kd_ref(vals[0], vals[2], vals[3], g=64 * one / 11)
+    for fuse in (True, False):
+        got = th.function([x, t, teacher, ids], th.grad(cost, x), fuse=fuse)(*vals)
+        # each gradient is rounded to float16, then their sum
+        off = 2.0 ** -11 * (np.abs(a["dx"][0]) + np.abs(b["dx"][0])) + 2 * 2.0 ** -25
+        close(got, a["dx"][0] + b["dx"][0], a["dx"][1] + b["dx"][1] + off / (chain(777) * 2.0 ** -24), chain(777), "dx", "float32")
 
 
 def test_second_derivatives_of_layer_normalization():

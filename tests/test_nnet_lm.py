@@ -106,15 +106,13 @@ def test_gradient_graphs(dry_run):
     assert names.count("HipLayerNormalization") == 1 and names.count("HipLayerNormalizationGrad") == 1
     t, w = T.lvector(), T.fvector()
     lp, h, tv, ti = nnet.token_log_probs(x, t, n_top=3)
-    f = th.function([x, t, w], th.grad(None, x, known_grads={lp: w}))
+    f = th.function([x, t, w], th.grad(None, x, known_grads={lp: w}), fuse=False)
     assert device_nodes(f) == ["HipTokenLogProbs", "HipTokenLogProbsGrad"]
     assert f.toposort()[-2].op.given == (True, False, False)
-    f = th.function([x, t, w], th.grad(None, x, known_grads={h: w}))
+    f = th.function([x, t, w], th.grad(None, x, known_grads={h: w}), fuse=False)
     assert f.toposort()[-2].op.given == (False, True, False)
     ids, teacher = T.imatrix(), T.fmatrix()
     loss = nnet.topk_distillation_loss(x, teacher, ids)
-    f = th.function([x, teacher, ids, w], th.grad(None, x, known_grads={loss: w}))
-    assert device_nodes(f) == ["HipTopKDistillation", "HipTopKDistillationGrad"]
     with pytest.raises(DisconnectedInputError):
         th.grad(T.sum(loss), teacher)
     with pytest.raises(DisconnectedInputError):
@@ -126,6 +124,38 @@ def test_gradient_graphs(dry_run):
     # equal calls on the same variables are one node
     f = th.function([x, t], [nnet.token_log_probs(x, t)[0], nnet.token_log_probs(x, t)[1]])
     assert device_nodes(f) == ["HipTokenLogProbs"]
+
+
+def test_one_launch_for_a_loss_and_its_gradient(dry_run):
+    """Gradients of the results that do not depend on the results are known before the launch."""
+    x, t, w = T.fmatrix(), T.lvector(), T.fvector()
+    ids, teacher = T.imatrix(), T.fmatrix()
+    lp, h = nnet.token_log_probs(x, t)
+    kd = nnet.topk_distillation_loss(x, teacher, ids)
+
+    def names(cost, **kw):
+        ins = [x, t, w, ids, teacher]
+        f = th.function(ins, [cost, th.grad(cost, x)], on_unused_input="ignore", **kw)
+        return [n for n in device_nodes(f) if "Token" in n or "TopK" in n]
+
+    for cost in (T.sum(-w * lp), T.mean(-lp), -T.sum(w * lp) / T.sum(w), T.sum(w * lp + np.float32(0.1) * h), T.mean(h),
+                 T.sum(w * lp) + T.mean(T.exp(w) * h)):
+        assert names(cost) == ["HipTokenLogProbsTrain"], cost
+        assert names(cost, fuse=False) == ["HipTokenLogProbs", "HipTokenLogProbsGrad"]
+    for cost in (T.sum(w * kd), T.mean(kd), T.sum(kd)):
+        assert names(cost) == ["HipTopKDistillationTrain"], cost
+    # the mean's weight is read as one value for all rows
+    f = th.function([x, teacher, ids], th.grad(T.mean(kd), x))
+    node = [n for n in f.toposort() if type(n.op).__name__ == "HipTopKDistillationTrain"][0]
+    assert node.inputs[3].type.broadcastable == (True,)
+    f(np.zeros((3, 5), "float32"), np.zeros((3, 2), "float32"), np.zeros((3, 2), "int32"))
+    # functions of the results themselves are not
+    for cost in (T.sum(T.exp(lp - w)), T.sum(lp * h), T.sum(T.sqr(h))):
+        assert names(cost) == ["HipTokenLogProbs", "HipTokenLogProbsGrad"], cost
+    assert names(T.sum(T.sqr(kd))) == ["HipTopKDistillation", "HipTopKDistillationGrad"]
+    assert names(T.sum(w * lp) + T.sum(T.sqr(kd))) == ["HipTokenLogProbsTrain", "HipTopKDistillation", "HipTopKDistillationGrad"]
+    # both losses of one batch of logits
+    assert sorted(names(T.sum(w * lp) + T.mean(kd))) == ["HipTokenLogProbsTrain", "HipTopKDistillationTrain"]
 
 
 def test_shapes_that_do_not_fit(dry_run):

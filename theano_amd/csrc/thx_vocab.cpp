@@ -402,34 +402,46 @@ struct KdRow {
   A *loss, *stats;
 };
 
+// Entry k of the teacher into its sums: nothing where it stands for no token, NaN where it names one that is not there,
+// which makes the row's loss and gradient NaN.
+template <class A>
+THX_DEV void take_entry(const Teacher<A>& t, int64_t r, int k, int64_t cols, A c, LaneSums<A, false>& ts) {
+  const int64_t id = load_index(t.ids, t.i64, r * t.is + k);
+  if (id < 0) return;
+  const A v = load_real<A>(t.logits, t.dtype, r * t.ls + k);
+  if (v > ts.m) ts.raise(v, c);
+  ts.add(v, c);
+  if (id >= cols) ts.s = (A)NAN;
+}
+
+// q (log q - log p) of an entry with logit v and token id >= 0; 0 where q is.
+template <class T, class A>
+THX_DEV A entry_loss(const KdRow<T>& q, A v, int64_t id, const T* x, int64_t cols, A c, const LaneSums<T, false>& sum, A ls,
+                     A tm, A tls) {
+  if (tm == neg_inf<A>() && tls == neg_inf<A>()) return 0;
+  const A p = acc_exp2((v - tm) * c - tls);
+  if (p == (A)0) return 0;
+  if (id >= cols) return (A)NAN;
+  const A lp = sum.nothing_left() ? neg_inf<A>() : log_prob(x[id], sum.m, c, q.inv_t, ls);
+  return p * (log_prob(v, tm, c, q.inv_t, tls) - lp);
+}
+
 template <class T>
 THX_DEV void finish(const KdRow<T>& q, const T* x, int64_t cols, int64_t r, typename AccOf<T>::type c,
                     const LaneSums<T, false>& sum) {
   typedef typename AccOf<T>::type A;
   const Teacher<A>& t = q.t;
   const int lane = threadIdx.x & 63;
-  const bool none = sum.nothing_left();
   const A ls = sum.log2_sum();
   LaneSums<A, false> ts;  // the teacher's side: entries as single or double precision
   ts.init();
-  for (int k = lane; k < t.n; k += 64) {
-    if (load_index(t.ids, t.i64, r * t.is + k) < 0) continue;
-    const A v = load_real<A>(t.logits, t.dtype, r * t.ls + k);
-    if (v > ts.m) ts.raise(v, c);
-    ts.add(v, c);
-  }
+  for (int k = lane; k < t.n; k += 64) take_entry(t, r, k, cols, c, ts);
   ts.join_lanes(c);
-  const bool tnone = ts.nothing_left();
   const A tls = ts.log2_sum();
   A loss = 0;
   for (int k = lane; k < t.n; k += 64) {
     const int64_t id = load_index(t.ids, t.i64, r * t.is + k);
-    if (id < 0) continue;
-    if (id >= cols) loss = (A)NAN;
-    if (id >= cols || tnone) continue;
-    const A v = load_real<A>(t.logits, t.dtype, r * t.ls + k), p = acc_exp2((v - ts.m) * c - tls);
-    const A lp = none ? neg_inf<A>() : log_prob(x[id], sum.m, c, q.inv_t, ls);
-    if (!(p == (A)0)) loss += p * (log_prob(v, ts.m, c, q.inv_t, tls) - lp);
+    if (id >= 0) loss += entry_loss(q, load_real<A>(t.logits, t.dtype, r * t.ls + k), id, x, cols, c, sum, ls, ts.m, tls);
   }
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) loss += __shfl_xor(loss, k, 64);
@@ -561,6 +573,7 @@ template <class A> struct Slope { A m, ls, a, b; };
 
 template <class A>
 struct LpGrad {
+  enum { kEntries = THX_MAX_TOP + 1 };
   const void* tokens; int64_t ts; int t64;
   const A* stats; int64_t ss;
   const A* entropy; int64_t es;
@@ -596,6 +609,7 @@ struct LpGrad {
 
 template <class A>
 struct KdGrad {
+  enum { kEntries = THX_MAX_TEACHER };
   Teacher<A> t;
   const A* stats; int64_t ss;
   const A* g; int64_t gs;
@@ -606,15 +620,12 @@ struct KdGrad {
     const A* st = stats + r * ss;
     const A tm = st[2], tls = st[3], gt = g[r * gs] * temperature;
     const bool tnone = tm == neg_inf<A>() && tls == neg_inf<A>();
-    bool beyond = false;
     for (int k = threadIdx.x; k < t.n; k += blockDim.x) {
       const int64_t j = load_index(t.ids, t.i64, r * t.is + k);
-      beyond |= j >= cols;
       id[k] = j >= 0 && j < cols && !tnone ? (int)j : -1;
       val[k] = -gt * acc_exp2((load_real<A>(t.logits, t.dtype, r * t.ls + k) - tm) * c - tls);
     }
-    const bool bad = __syncthreads_or(beyond);
-    return {st[0], st[1], bad ? (A)NAN : tnone ? (A)0 : gt, (A)0};
+    return {st[0], st[1], tls != tls ? tls : tnone ? (A)0 : gt, (A)0};
   }
 };
 
@@ -629,28 +640,80 @@ struct GradCut {
   T* dx;
 };
 
+
+// The slope of a row's elements.
+template <class T>
+struct RowSlope {
+  typedef typename AccOf<T>::type A;
+  LaneSums<T, false> at;
+  A a, b, c;
+  bool none;
+  THX_DEV RowSlope(const Slope<A>& s, A c_) : c(c_) {
+    none = s.m == neg_inf<A>() && s.ls == neg_inf<A>();
+    at.ref = none ? (A)0 : sizeof(T) == 2 ? product(s.m, c) : s.m;
+    const A inv = none ? (A)0 : acc_exp2(-s.ls);
+    a = none ? (A)0 : (s.a - s.b * s.ls) * inv;
+    b = s.b * inv;
+  }
+  THX_DEV A operator()(T v) const { return b == (A)0 ? of<false>(v) : of<true>(v); }
+  template <bool B>
+  THX_DEV A of(T v) const {
+    const A d = at.exponent((A)v, c), e = acc_exp2(d);
+    return B ? e * (a + b * LaneSums<T, false>::bounded(d)) : e * a;
+  }
+  // In place, over N vectors; whether there is a b is the same for the whole row.
+  template <int V, int N>
+  THX_DEV void over(Vec<T, V> (&v)[N]) const {
+    if (none) {
+#pragma unroll
+      for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[u].v[e] = (T)0;
+    } else if (b == (A)0) {
+#pragma unroll
+      for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[u].v[e] = (T)of<false>(v[u].v[e]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[u].v[e] = (T)of<true>(v[u].v[e]);
+    }
+  }
+};
+
+// The elements of columns [first, last) that the list names, written over; behind a barrier.
+template <class T, class A>
+THX_DEV void write_entries(const RowSlope<T>& slope, const T* x, T* dx, const int* id, const A* val, int n, int64_t first,
+                           int64_t last) {
+  for (int k = threadIdx.x; k < n; k += blockDim.x) {
+    const int j = id[k];
+    if (j < first || j >= last) continue;
+    A v = 0;
+    bool mine = true;
+    for (int i = 0; i < n; ++i)
+      if (id[i] == j) {
+        v += val[i];
+        if (i < k) mine = false;
+      }
+    if (mine) dx[j] = (T)(slope(x[j]) + v);
+  }
+}
+
 template <class T, class Row>
 __global__ void __launch_bounds__(256) vocab_grad(GradCut<T> q, Row row) {
   typedef typename AccOf<T>::type A;
   constexpr int V = Width<T>::value;
-  __shared__ int id[THX_MAX_TEACHER];
-  __shared__ A val[THX_MAX_TEACHER];
+  __shared__ int id[Row::kEntries];
+  __shared__ A val[Row::kEntries];
   const int64_t units = q.rows * q.segs, whole = q.cols / V, vectors = (q.cols + V - 1) / V;
   for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
     const int64_t r = unit / q.segs, seg = unit - r * q.segs;
     const T* x = q.x + r * q.xs;
     T* dx = q.dx + r * q.cols;
-    const Slope<A> s = row.open(r, q.cols, id, val);
-    const bool none = s.m == neg_inf<A>() && s.ls == neg_inf<A>();
-    LaneSums<T, false> at;
-    at.ref = none ? (A)0 : sizeof(T) == 2 ? product(s.m, q.c) : s.m;
-    const A inv = none ? (A)0 : acc_exp2(-s.ls);
-    const A a = none ? (A)0 : (s.a - s.b * s.ls) * inv, b = s.b * inv;
+    const RowSlope<T> slope(row.open(r, q.cols, id, val), q.c);
     const int64_t lo = seg * q.per, hi = lo + q.per < vectors ? lo + q.per : vectors;
-    auto slope = [&](T v) {
-      const A d = at.exponent((A)v, q.c), e = acc_exp2(d);
-      return b == (A)0 ? e * a : e * (a + b * LaneSums<T, false>::bounded(d));
-    };
     for (int64_t i0 = lo; i0 < hi; i0 += 256 * kUnroll) {
       Vec<T, V> v[kUnroll];
 #pragma unroll
@@ -658,36 +721,192 @@ __global__ void __launch_bounds__(256) vocab_grad(GradCut<T> q, Row row) {
         const int64_t i = i0 + u * 256 + threadIdx.x;
         if (i < hi && i < whole) load_vec<T, V, false, true>(v[u], x + i * V);
       }
+      slope.over(v);
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         const int64_t i = i0 + u * 256 + threadIdx.x;
         if (i < hi && i < whole) {
-#pragma unroll
-          for (int e = 0; e < V; ++e) v[u].v[e] = none ? (T)0 : (T)slope(v[u].v[e]);
           store_vec<T, V, false, true>(dx + i * V, v[u]);
         } else if (i < hi) {
-          for (int64_t j = i * V; j < q.cols; ++j) dx[j] = none ? (T)0 : (T)slope(x[j]);
+          for (int64_t j = i * V; j < q.cols; ++j) dx[j] = slope.none ? (T)0 : (T)slope(x[j]);
         }
       }
     }
     __syncthreads();  // the entries are there, and the elements they replace are written
-    if (!none) {
-      const int n = row.entries();
-      const int64_t first = lo * V, last = hi * V;
-      for (int k = threadIdx.x; k < n; k += 256) {
-        const int j = id[k];
-        if (j < first || j >= last) continue;
-        A v = 0;
-        bool mine = true;
-        for (int i = 0; i < n; ++i)
-          if (id[i] == j) {
-            v += val[i];
-            if (i < k) mine = false;
-          }
-        if (mine) dx[j] = (T)(slope(x[j]) + v);
+    if (!slope.none) write_entries(slope, x, dx, id, val, row.entries(), lo * V, hi * V);
+    __syncthreads();  // before the next row's entries
+  }
+}
+
+// ---- forward and gradient in one ---------------------------------------------------------------------------------------
+//
+// Where the gradients of a row's results are known beforehand (the weight of a loss), one block reads the row once, keeps
+// it in registers through the sums, and writes the gradient from there: two passes over memory instead of three.
+
+template <class T>
+struct LpTrain {
+  typedef typename AccOf<T>::type A;
+  enum { kEntries = 1, kEntropy = 1 };
+  LpRow<T> out;
+  const A* g; int64_t gs;
+  const A* u; int64_t us;
+};
+
+template <class T>
+struct KdTrain {
+  typedef typename AccOf<T>::type A;
+  enum { kEntries = THX_MAX_TEACHER, kEntropy = 0 };
+  KdRow<T> out;
+  const A* g; int64_t gs;
+  A temperature;
+};
+
+// The compiler forgets what it knows about a vector's values: without this it keeps single-precision copies of a row's
+// elements from the first use to the second, which is twice the registers.
+template <class T, int V>
+THX_DEV void forget(Vec<T, V>& v) {
+  thx_u32x4& raw = *(thx_u32x4*)&v;
+  asm volatile("" : "+v"(raw));
+}
+
+template <class T, class Row, int THREADS, int VPT>
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 8 && sizeof(T) < 8 ? 8 : 1)
+vocab_train(GradCut<T> q, Row row) {
+  typedef typename AccOf<T>::type A;
+  constexpr int V = Width<T>::value, W = THREADS / 64;
+  constexpr bool ENT = Row::kEntropy;
+  constexpr int G = VPT % 4 ? (VPT % 2 ? 1 : 2) : 4;  // vectors between two looks at the maximum
+  __shared__ int id[Row::kEntries];
+  __shared__ A val[Row::kEntries];
+  __shared__ A part[W][ENT ? 3 : 4], losses[W];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+  // rounds that every thread takes part in, and the vectors and elements that are left
+  const int whole = (int)(q.cols / V), full = whole / THREADS, rest = (int)(q.cols - (int64_t)whole * V);
+  for (int64_t r = blockIdx.x; r < q.rows; r += gridDim.x) {
+    const T* x = q.x + r * q.xs;
+    T* dx = q.dx + r * q.cols;
+    const T* xt = x + (int)threadIdx.x * V;
+    Vec<T, V> v[VPT];
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      if (u < full) {
+        load_vec<T, V, false, true>(v[u], xt + u * (THREADS * V));
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[u].v[e] = (T)neg_inf<A>();
+        if (u == full && u * THREADS + (int)threadIdx.x < whole) load_vec<T, V, false, true>(v[u], xt + u * (THREADS * V));
       }
     }
-    __syncthreads();  // before the next row's entries
+    // the elements behind the last whole vector, one to a thread
+    const bool extra = (int)threadIdx.x < rest;
+    const T tail = extra ? x[(int64_t)whole * V + threadIdx.x] : (T)neg_inf<A>();
+    LaneSums<T, ENT> sum;
+    sum.init();
+    if ((A)tail > sum.m) sum.raise((A)tail, q.c);
+    sum.add((A)tail, q.c);
+#pragma unroll
+    for (int u = 0; u < VPT; u += G) {
+      if (u > full) continue;
+      A m = vector_max(v[u]);
+#pragma unroll
+      for (int k = 1; k < G; ++k) {
+        const A o = vector_max(v[u + k]);
+        m = m > o ? m : o;
+      }
+      if (m > sum.m) sum.raise(m, q.c);
+#pragma unroll
+      for (int k = 0; k < G; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum.add((A)v[u + k].v[e], q.c);
+    }
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) forget(v[u]);
+    sum.join_lanes(q.c);
+    if (lane == 0) {
+      part[wave][0] = sum.m, part[wave][1] = sum.s;
+      if constexpr (ENT) part[wave][2] = sum.w;
+    }
+    [[maybe_unused]] LaneSums<A, false> ts;
+    if constexpr (!ENT) {
+      ts.init();
+      for (int k = threadIdx.x; k < row.out.t.n; k += THREADS) take_entry(row.out.t, r, k, q.cols, q.c, ts);
+      ts.join_lanes(q.c);
+      if (lane == 0) part[wave][2] = ts.m, part[wave][3] = ts.s;
+    }
+    __syncthreads();
+    sum.init();
+    if constexpr (!ENT) ts.init();
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      sum.join(part[w][0], part[w][1], ENT ? part[w][2] : (A)0, q.c);
+      if constexpr (!ENT) ts.join(part[w][2], part[w][3], (A)0, q.c);
+    }
+    const A ls = sum.log2_sum();
+    Slope<A> s = {sum.m, ls, (A)0, (A)0};
+    int n;
+    if constexpr (ENT) {
+      const LpRow<T>& o = row.out;
+      n = 1;
+      const int64_t t = load_index(o.tokens, o.t64, r * o.ts);
+      const A w = row.g && t >= 0 ? row.g[r * row.gs] : (A)0, h = row.u ? row.u[r * row.us] : (A)0;
+      const A entropy = sum.nothing_left() ? (A)0 : (ls - sum.w / sum.s) * (A)kLn2;
+      s.a = -((t >= q.cols && row.g ? (A)NAN : w) + (row.u ? h * entropy : (A)0)) * o.inv_t;
+      s.b = -h * (A)kLn2 * o.inv_t;
+      if (threadIdx.x == 0) {
+        id[0] = row.g && t >= 0 && t < q.cols ? (int)t : -1;
+        val[0] = w * o.inv_t;
+        A lp = 0;
+        if (t >= q.cols) lp = (A)NAN;
+        else if (t >= 0) lp = sum.nothing_left() ? neg_inf<A>() : log_prob(x[t], sum.m, q.c, o.inv_t, ls);
+        o.o.log_prob[r] = lp;
+        o.o.entropy[r] = entropy;
+        o.o.stats[2 * r] = sum.m;
+        o.o.stats[2 * r + 1] = ls;
+      }
+    } else {
+      const KdRow<T>& o = row.out;
+      const Teacher<A>& t = o.t;
+      n = t.n;
+      const A tls = ts.log2_sum(), gt = row.g[r * row.gs] * row.temperature;
+      s.a = tls != tls ? tls : ts.nothing_left() ? (A)0 : gt;
+      A loss = 0;
+      for (int k = threadIdx.x; k < n; k += THREADS) {
+        const int64_t j = load_index(t.ids, t.i64, r * t.is + k);
+        const A e = load_real<A>(t.logits, t.dtype, r * t.ls + k);
+        id[k] = j >= 0 && j < q.cols && !ts.nothing_left() ? (int)j : -1;
+        val[k] = -gt * acc_exp2((e - ts.m) * q.c - tls);
+        if (j >= 0) loss += entry_loss(o, e, j, x, q.cols, q.c, sum, ls, ts.m, tls);
+      }
+#pragma unroll
+      for (int k = 1; k < 64; k <<= 1) loss += __shfl_xor(loss, k, 64);
+      if (lane == 0) losses[wave] = loss;
+      if (threadIdx.x == 0) {
+        o.stats[4 * r] = sum.m;
+        o.stats[4 * r + 1] = ls;
+        o.stats[4 * r + 2] = ts.m;
+        o.stats[4 * r + 3] = tls;
+      }
+    }
+    const RowSlope<T> slope(s, q.c);
+    T* dt = dx + (int)threadIdx.x * V;
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      if (u > full) continue;
+      Vec<T, V> o[1] = {v[u]};
+      slope.over(o);
+      if (u < full || u * THREADS + (int)threadIdx.x < whole) store_vec<T, V, false, true>(dt + u * (THREADS * V), o[0]);
+    }
+    if (extra) dx[(int64_t)whole * V + threadIdx.x] = slope.none ? (T)0 : (T)slope(tail);
+    __syncthreads();  // the entries and the losses are there, and the elements that the entries replace are written
+    if (!slope.none) write_entries(slope, x, dx, id, val, n, 0, q.cols);
+    if constexpr (!ENT) {
+      if (threadIdx.x == 0) {
+        A loss = losses[0];
+        for (int w = 1; w < W; ++w) loss += losses[w];
+        row.out.loss[r] = (sum.s != sum.s ? sum.s : loss) * row.out.t2;
+      }
+    }
+    __syncthreads();  // before the next row's
   }
 }
 
@@ -744,8 +963,9 @@ int launch_forward(Cut<T> q, Row row, const std::string& plan) {
   return launch_builtin((const void*)&vocab_join<T, TOP, Row, ENT>, plan + "|join", dim3(grid_of(q.rows)), dim3(64), args);
 }
 
-// The gradient's segments: blocks of 256 threads, at most kUnroll vectors to a thread, and fewer where that leaves
-// compute units without work.
+// The gradient's segments: 16 blocks to a compute unit where there are too few rows for that, one vector to a thread at
+// least; whole rows else, since every segment reads the row's list again (2048 rows of 32000 floats, 64 entries: 153 us
+// in segments of 4 vectors to a thread, 116 us in two segments a row).
 template <class T, class Row>
 int launch_grad(const Rows& x, double temperature, char* dx, Row row, const std::string& plan) {
   typedef typename AccOf<T>::type A;
@@ -753,14 +973,53 @@ int launch_grad(const Rows& x, double temperature, char* dx, Row row, const std:
   const int64_t vectors = ceil_div(x.cols, Width<T>::value);
   q.x = (const T*)x.ptr;
   q.xs = x.stride, q.rows = x.rows, q.cols = x.cols;
-  q.segs = (int)ceil_div(vectors, 256 * kUnroll);
-  if (x.rows * q.segs < 4 * compute_units())
-    q.segs = (int)std::max<int64_t>(q.segs, std::min<int64_t>(ceil_div(vectors, 256), ceil_div(4 * compute_units(), x.rows)));
+  q.segs = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(vectors, 256), ceil_div(16 * compute_units(), x.rows)));
   q.per = ceil_div(vectors, q.segs);
   q.c = (A)(kLog2E / temperature);
   q.dx = (T*)dx;
   void* args[] = {&q, &row};
   return launch_builtin((const void*)&vocab_grad<T, Row>, plan, dim3(grid_of(x.rows * q.segs)), dim3(256), args);
+}
+
+// The block that holds a row of the one-pass kernel: threads, and vectors to a thread; 0 where none does.
+struct Hold {
+  int threads = 0, vpt = 0;
+};
+Hold hold_of(const Rows& x) {
+  static const Hold all[] = {{256, 1}, {256, 2}, {256, 4}, {256, 8}, {512, 8}, {1024, 8}, {1024, 16}, {1024, 20}};
+  const int isz = dtype_size(x.dtype);
+  const int64_t whole = x.cols / (16 / isz);  // the elements behind the last whole vector go to one thread each
+  for (const Hold& h : all)
+    if (whole <= (int64_t)h.threads * h.vpt && !(isz == 8 && h.vpt > 8)) return h;
+  return Hold();
+}
+
+std::string held_plan(const char* name, const Rows& x, const Hold& h) {
+  return std::string(name) + "|t" + std::to_string(x.dtype) + "|r" + std::to_string(h.threads) + "x" + std::to_string(h.vpt);
+}
+
+template <class T, class Row>
+int launch_train(const Rows& x, double temperature, char* dx, const Hold& h, Row row, const std::string& plan) {
+  typedef typename AccOf<T>::type A;
+  GradCut<T> q = {};
+  q.x = (const T*)x.ptr;
+  q.xs = x.stride, q.rows = x.rows, q.cols = x.cols;
+  q.c = (A)(kLog2E / temperature);
+  q.dx = (T*)dx;
+  void* args[] = {&q, &row};
+  const void* kernel = nullptr;
+  switch (h.threads * 32 + h.vpt) {
+    case 256 * 32 + 1: kernel = (const void*)&vocab_train<T, Row, 256, 1>; break;
+    case 256 * 32 + 2: kernel = (const void*)&vocab_train<T, Row, 256, 2>; break;
+    case 256 * 32 + 4: kernel = (const void*)&vocab_train<T, Row, 256, 4>; break;
+    case 256 * 32 + 8: kernel = (const void*)&vocab_train<T, Row, 256, 8>; break;
+    case 512 * 32 + 8: kernel = (const void*)&vocab_train<T, Row, 512, 8>; break;
+    case 1024 * 32 + 8: kernel = (const void*)&vocab_train<T, Row, 1024, 8>; break;
+    default:
+      if constexpr (sizeof(T) < 8)
+        kernel = h.vpt == 16 ? (const void*)&vocab_train<T, Row, 1024, 16> : (const void*)&vocab_train<T, Row, 1024, 20>;
+  }
+  return launch_builtin(kernel, plan, dim3(grid_of(x.rows)), dim3(h.threads), args);
 }
 
 template <class F>
@@ -788,6 +1047,16 @@ int indices_of(const char* what, const char* name, const thx_array* a, const thx
   const int dt = a->dtype & ~THX_REUSED;
   if (dt != THX_I32 && dt != THX_I64) return fail(THX_ERR_TYPE, "%s: %s must be int32 or int64", what, name);
   return like_rows(what, name, a, x, dt, cols, flags, r);
+}
+
+// The gradient of a result with one value per row: such values, or one value (every extent 1) for all rows.
+int row_gradient(const char* what, const char* name, const thx_array* a, const thx_array* x, int acc, int flags, Rows* r) {
+  bool one = a->nd == x->nd - 1;
+  for (int d = 0; one && d < a->nd; ++d) one = a->shape[d] == 1;
+  if (!one) return like_rows(what, name, a, x, acc, -1, flags, r);
+  int rc = rows_of(what, name, a, acc, 0, flags, r);
+  r->stride = 0;
+  return rc;
 }
 
 int token_logprob(const thx_array* logits, const thx_array* tokens, double temperature, int n_top, const thx_array* log_prob,
@@ -847,8 +1116,8 @@ int token_logprob_grad(const thx_array* logits, const thx_array* tokens, const t
   if ((rc = indices_of(what, "tokens", tokens, logits, -1, flags, &in[1]))) return rc;
   if ((rc = like_rows(what, "stats", stats, logits, acc, 2, flags, &in[2]))) return rc;
   if ((rc = like_rows(what, "entropy", entropy, logits, acc, -1, flags, &in[3]))) return rc;
-  if (g && (rc = like_rows(what, "g_log_prob", g, logits, acc, -1, flags, &in[5]))) return rc;
-  if (u && (rc = like_rows(what, "g_entropy", u, logits, acc, -1, flags, &in[6]))) return rc;
+  if (g && (rc = row_gradient(what, "g_log_prob", g, logits, acc, flags, &in[5]))) return rc;
+  if (u && (rc = row_gradient(what, "g_entropy", u, logits, acc, flags, &in[6]))) return rc;
   if ((rc = like_rows(what, "dlogits", dx, logits, in[0].dtype, in[0].cols, flags, &out))) return rc;
   if ((rc = contiguous_rows(what, "dlogits", out))) return rc;
   if ((rc = no_overlap(what, &out, 1, in, 8)) && !dry) return rc;
@@ -924,7 +1193,7 @@ int topk_distill_grad(const thx_array* logits, const thx_array* teacher, const t
   const int acc = acc_code(in[0].dtype);
   if ((rc = teacher_of(what, teacher, tokens, logits, flags, &in[1], &in[2]))) return rc;
   if ((rc = like_rows(what, "stats", stats, logits, acc, 4, flags, &in[3]))) return rc;
-  if ((rc = like_rows(what, "g_loss", g, logits, acc, -1, flags, &in[4]))) return rc;
+  if ((rc = !g ? fail(THX_ERR_ARG, "%s: g_loss is missing", what) : row_gradient(what, "g_loss", g, logits, acc, flags, &in[4]))) return rc;
   if ((rc = like_rows(what, "dlogits", dx, logits, in[0].dtype, in[0].cols, flags, &out))) return rc;
   if ((rc = contiguous_rows(what, "dlogits", out))) return rc;
   if ((rc = no_overlap(what, &out, 1, in, 5)) && !dry) return rc;
@@ -938,6 +1207,82 @@ int topk_distill_grad(const thx_array* logits, const thx_array* teacher, const t
     const KdGrad<A> row = {teacher_args<A>(in[1], in[2]), (const A*)in[3].ptr, in[3].stride, (const A*)in[4].ptr,
                            in[4].stride, (A)(kLog2E / temperature), (A)temperature};
     return launch_grad<T>(in[0], temperature, out.ptr, row, plan);
+  });
+}
+
+int token_logprob_train(const thx_array* logits, const thx_array* tokens, const thx_array* g, const thx_array* u,
+                        double temperature, const thx_array* log_prob, const thx_array* entropy, const thx_array* stats,
+                        const thx_array* dx, void* ws, size_t ws_bytes, int flags) {
+  const char* what = "token log probabilities with their gradient";
+  // the checks, and the two calls where no block holds a row
+  int rc = token_logprob(logits, tokens, temperature, 0, log_prob, entropy, nullptr, nullptr, stats, ws, ws_bytes,
+                         flags | THX_DRY_RUN);
+  if (!rc) rc = token_logprob_grad(logits, tokens, stats, entropy, nullptr, g, u, nullptr, temperature, dx, flags | THX_DRY_RUN);
+  if (rc) return rc;
+  Rows x, t, gr, ur, out[4];
+  if ((rc = logits_of(what, logits, temperature, flags, &x))) return rc;
+  const Hold h = hold_of(x);
+  if (!h.threads) {
+    rc = token_logprob(logits, tokens, temperature, 0, log_prob, entropy, nullptr, nullptr, stats, ws, ws_bytes, flags);
+    return rc ? rc : token_logprob_grad(logits, tokens, stats, entropy, nullptr, g, u, nullptr, temperature, dx, flags);
+  }
+  const int acc = acc_code(x.dtype);
+  if ((rc = indices_of(what, "tokens", tokens, logits, -1, flags, &t))) return rc;
+  if (g && (rc = row_gradient(what, "g_log_prob", g, logits, acc, flags, &gr))) return rc;
+  if (u && (rc = row_gradient(what, "g_entropy", u, logits, acc, flags, &ur))) return rc;
+  if ((rc = like_rows(what, "log_prob", log_prob, logits, acc, -1, flags, &out[0]))) return rc;
+  if ((rc = like_rows(what, "entropy", entropy, logits, acc, -1, flags, &out[1]))) return rc;
+  if ((rc = like_rows(what, "stats", stats, logits, acc, 2, flags, &out[2]))) return rc;
+  if ((rc = like_rows(what, "dlogits", dx, logits, x.dtype, x.cols, flags, &out[3]))) return rc;
+  const Rows ins[] = {x, t, gr, ur};
+  if ((rc = no_overlap(what, out, 4, ins, 4)) && !(flags & THX_DRY_RUN)) return rc;
+  const std::string plan = held_plan("lpt", x, h);
+  set_last_plan(plan);
+  if ((flags & THX_DRY_RUN) || !x.rows) return THX_OK;
+  if ((rc = ensure_init())) return rc;
+  return by_type(x.dtype, [&](auto tag) {
+    typedef decltype(tag) T;
+    typedef typename AccOf<T>::type A;
+    const LpTrain<T> row = {{t.ptr, t.stride, t.dtype == THX_I64, 0, (A)(1.0 / temperature),
+                             {(A*)out[0].ptr, (A*)out[1].ptr, nullptr, nullptr, (A*)out[2].ptr}},
+                            (const A*)gr.ptr, gr.stride, (const A*)ur.ptr, ur.stride};
+    return launch_train<T>(x, temperature, out[3].ptr, h, row, plan);
+  });
+}
+
+int topk_distill_train(const thx_array* logits, const thx_array* teacher, const thx_array* tokens, const thx_array* g,
+                       double temperature, const thx_array* loss, const thx_array* stats, const thx_array* dx, void* ws,
+                       size_t ws_bytes, int flags) {
+  const char* what = "distillation loss with its gradient";
+  int rc = topk_distill(logits, teacher, tokens, temperature, loss, stats, ws, ws_bytes, flags | THX_DRY_RUN);
+  if (!rc) rc = topk_distill_grad(logits, teacher, tokens, stats, g, temperature, dx, flags | THX_DRY_RUN);
+  if (rc) return rc;
+  Rows x, t, ids, gr, out[3];
+  if ((rc = logits_of(what, logits, temperature, flags, &x))) return rc;
+  const Hold h = hold_of(x);
+  if (!h.threads) {
+    rc = topk_distill(logits, teacher, tokens, temperature, loss, stats, ws, ws_bytes, flags);
+    return rc ? rc : topk_distill_grad(logits, teacher, tokens, stats, g, temperature, dx, flags);
+  }
+  const int acc = acc_code(x.dtype);
+  if ((rc = teacher_of(what, teacher, tokens, logits, flags, &t, &ids))) return rc;
+  if ((rc = row_gradient(what, "g_loss", g, logits, acc, flags, &gr))) return rc;
+  if ((rc = like_rows(what, "loss", loss, logits, acc, -1, flags, &out[0]))) return rc;
+  if ((rc = like_rows(what, "stats", stats, logits, acc, 4, flags, &out[1]))) return rc;
+  if ((rc = like_rows(what, "dlogits", dx, logits, x.dtype, x.cols, flags, &out[2]))) return rc;
+  const Rows ins[] = {x, t, ids, gr};
+  if ((rc = no_overlap(what, out, 3, ins, 4)) && !(flags & THX_DRY_RUN)) return rc;
+  const std::string plan = held_plan("kdt", x, h);
+  set_last_plan(plan);
+  if ((flags & THX_DRY_RUN) || !x.rows) return THX_OK;
+  if ((rc = ensure_init())) return rc;
+  return by_type(x.dtype, [&](auto tag) {
+    typedef decltype(tag) T;
+    typedef typename AccOf<T>::type A;
+    const KdTrain<T> row = {{teacher_args<A>(t, ids), (A)(1.0 / temperature), (A)(temperature * temperature),
+                             (A*)out[0].ptr, (A*)out[1].ptr},
+                            (const A*)gr.ptr, gr.stride, (A)temperature};
+    return launch_train<T>(x, temperature, out[2].ptr, h, row, plan);
   });
 }
 
@@ -1001,6 +1346,26 @@ int thx_topk_distill_grad_call(const thx_array* logits, const thx_array* teacher
                                const thx_array* dlogits, int flags) {
   return guarded("thx_topk_distill_grad_call",
                  [&] { return topk_distill_grad(logits, teacher, tokens, stats, g_loss, temperature, dlogits, flags); });
+}
+
+int thx_token_logprob_train_call(const thx_array* logits, const thx_array* tokens, const thx_array* g_log_prob,
+                                 const thx_array* g_entropy, double temperature, const thx_array* log_prob,
+                                 const thx_array* entropy, const thx_array* stats, const thx_array* dlogits,
+                                 void* workspace, size_t workspace_bytes, int flags) {
+  return guarded("thx_token_logprob_train_call", [&] {
+    return token_logprob_train(logits, tokens, g_log_prob, g_entropy, temperature, log_prob, entropy, stats, dlogits,
+                               workspace, workspace_bytes, flags);
+  });
+}
+
+int thx_topk_distill_train_call(const thx_array* logits, const thx_array* teacher, const thx_array* tokens,
+                                const thx_array* g_loss, double temperature, const thx_array* loss,
+                                const thx_array* stats, const thx_array* dlogits, void* workspace,
+                                size_t workspace_bytes, int flags) {
+  return guarded("thx_topk_distill_train_call", [&] {
+    return topk_distill_train(logits, teacher, tokens, g_loss, temperature, loss, stats, dlogits, workspace,
+                              workspace_bytes, flags);
+  });
 }
 
 }  // extern "C"

@@ -8,8 +8,11 @@ import ctypes
 
 import numpy as np
 
-from ..gof import Apply
+from .. import scalar as scal
+from ..gof import Apply, Op
+from ..tensor import basic as T
 from ..tensor import nnet_lm as L
+from ..tensor.elemwise import DimShuffle, Elemwise
 from ..tensor.type import TensorType
 from .ops import HipArrayType, as_hip_variable
 from .runtime import HipArray, _Buffer, call_flags, check, lib, mark_reused, thx_array
@@ -131,6 +134,173 @@ class HipTopKDistillationGrad(_RowOp, L.TopKDistillationGrad):
     def call(self, node, ins, outs, flags):
         return lib.thx_topk_distill_grad_call(_at(ins, 0), _at(ins, 1), _at(ins, 2), _at(ins, 3), _at(ins, 4),
                                               self.temperature, _at(outs, 0), flags)
+
+
+class _TrainOp(_RowOp):
+    """A forward operator and its gradient in one launch, for gradients of the result that do not depend on the result:
+    what ``fuse_known_gradients`` makes of the two nodes.  There is no host counterpart."""
+
+    def make_node(self, *inputs):
+        ins = [as_hip_variable(i) for i in inputs]
+        n = self.n_forward
+        outs = self.forward.make_node(*ins[:n]).outputs
+        acc = outs[0].type.dtype
+        for g in ins[n:]:
+            if g.type.dtype != acc or g.type.ndim != ins[0].type.ndim - 1:
+                raise TypeError("%s: a gradient of type %s" % (self, g.type))
+        return Apply(self, ins, [o.type() for o in outs] + [ins[0].type()])
+
+    def infer_shape(self, node, shapes):
+        return self.forward.infer_shape(node, shapes[:self.n_forward]) + [shapes[0]]
+
+
+class HipTokenLogProbsTrain(_TrainOp, Op):
+    """``HipTokenLogProbs`` without alternatives and ``HipTokenLogProbsGrad``; ``given`` says which of the gradients of
+    ``log_prob`` and ``entropy`` follow the logits and the tokens."""
+
+    __props__ = ("temperature", "given")
+    n_forward = 2
+
+    def __init__(self, temperature, given):
+        self.temperature, self.given = float(temperature), tuple(bool(g) for g in given)
+        self.forward = HipTokenLogProbs(0, temperature)
+
+    def call(self, node, ins, outs, flags):
+        rc, ws, size = self.workspace(node, ins, lib.thx_token_logprob_workspace, 0)
+        at = iter(range(2, len(node.inputs)))
+        g, u = [next(at) if there else None for there in self.given]
+        return rc or lib.thx_token_logprob_train_call(_at(ins, 0), _at(ins, 1), _at(ins, g), _at(ins, u), self.temperature,
+                                                      _at(outs, 0), _at(outs, 1), _at(outs, 2), _at(outs, 3),
+                                                      ws.ptr if ws else None, size, flags)
+
+
+class HipTopKDistillationTrain(_TrainOp, Op):
+    """``HipTopKDistillation`` and ``HipTopKDistillationGrad``; the gradient of the loss follows the teacher's tokens."""
+
+    __props__ = ("temperature",)
+    n_forward = 3
+
+    def __init__(self, temperature):
+        self.temperature = float(temperature)
+        self.forward = HipTopKDistillation(temperature)
+
+    def call(self, node, ins, outs, flags):
+        rc, ws, size = self.workspace(node, ins, lib.thx_topk_distill_workspace)
+        return rc or lib.thx_topk_distill_train_call(_at(ins, 0), _at(ins, 1), _at(ins, 2), _at(ins, 3), self.temperature,
+                                                     _at(outs, 0), _at(outs, 1), _at(outs, 2), ws.ptr if ws else None,
+                                                     size, flags)
+
+
+class _Apart(object):
+    """Rewrites expressions so that they no longer depend on the results of one node, where all they take from them is
+    their shape: the fills that sums and means leave in gradients."""
+
+    def __init__(self, node, rows):
+        self.node, self.rows = node, rows     # ``rows``: makes a variable with the shape of the node's results per row
+        self.known, self.model = {}, None
+
+    def depends(self, v):
+        if v not in self.known:
+            n = v.owner
+            self.known[v] = n is not None and (n is self.node or any(self.depends(i) for i in n.inputs))
+        return self.known[v]
+
+    def row_shaped(self, v):
+        """Elementwise over a result of the node, and nowhere broadcast against anything larger."""
+        first = self.node.outputs[0].type
+        n = v.owner
+        if n is None or v.type.broadcastable != first.broadcastable:
+            return False
+        return n is self.node or (isinstance(n.op, Elemwise) and any(self.row_shaped(i) for i in n.inputs))
+
+    def shape_of_rows(self):
+        if self.model is None:
+            self.model = self.rows()
+        return self.model
+
+    def __call__(self, v):
+        """``v`` without the dependence, or None."""
+        if not self.depends(v):
+            return v
+        n = v.owner
+        if n is self.node:
+            return None
+        if isinstance(n.op, T.ShapeFloat) and self.row_shaped(n.inputs[0]):
+            return n.op(self.shape_of_rows())
+        if isinstance(n.op, Elemwise) and isinstance(n.op.scalar_op, scal.Second):
+            value = self(n.inputs[1])
+            if value is None:
+                return None
+            if not self.depends(n.inputs[0]):
+                model = n.inputs[0]
+            elif self.row_shaped(n.inputs[0]):
+                model = self.shape_of_rows()
+            else:
+                return None
+            return n.op.make_node(model, value).outputs[0]
+        if isinstance(n.op, (Elemwise, DimShuffle)) and not getattr(n.op, "inplace_pattern", None):
+            ins = [self(i) for i in n.inputs]
+            if any(i is None for i in ins):
+                return None
+            return n.op.make_node(*ins).outputs[v.index]
+        return None
+
+
+def _one_value(g):
+    """The single value that a fill repeats over the rows, if it can be had without a launch or a transfer: such an
+    operand is read with a stride of 0."""
+    n = g.owner
+    if n is None or not isinstance(n.op, Elemwise) or not isinstance(n.op.scalar_op, scal.Second):
+        return g
+    v = n.inputs[1]
+    if v.type.ndim != g.type.ndim or not all(v.type.broadcastable) or v.type.dtype != g.type.dtype:
+        return g
+    return v if isinstance(v.type, HipArrayType) else g
+
+
+def fuse_known_gradients(fgraph):
+    """A forward node over the vocabulary and its gradient node become one where the gradients of the results do not
+    depend on the results: a weighted sum or mean of the losses, not a function such as a ratio of probabilities."""
+    count = 0
+    for node in fgraph.toposort():
+        if node not in fgraph.apply_nodes:
+            continue
+        if isinstance(node.op, HipTokenLogProbsGrad):
+            if node.op.given[2]:
+                continue
+            fwd, first = node.inputs[2].owner, 4
+            if fwd is None or not isinstance(fwd.op, HipTokenLogProbs) or fwd.op.n_top or node.inputs[3] is not fwd.outputs[1]:
+                continue
+            new_op = HipTokenLogProbsTrain(node.op.temperature, node.op.given[:2])
+            rows = lambda: fwd.inputs[1]                                                  # noqa: E731
+        elif isinstance(node.op, HipTopKDistillationGrad):
+            fwd, first = node.inputs[3].owner, 4
+            if fwd is None or not isinstance(fwd.op, HipTopKDistillation):
+                continue
+            new_op = HipTopKDistillationTrain(node.op.temperature)
+
+            def rows():     # the first entry of every row
+                from .views import HipSubtensor
+                ids = fwd.inputs[2]
+                return HipSubtensor((slice(None),) * (ids.type.ndim - 1) + (0,)).make_node(ids).outputs[0]
+        else:
+            continue
+        n = new_op.n_forward
+        if fwd.op.temperature != node.op.temperature or list(fwd.inputs) != list(node.inputs[:n]):
+            continue
+        apart = _Apart(fwd, rows)
+        gs = [apart(g) for g in node.inputs[first:]]
+        if any(g is None for g in gs):
+            continue
+        new = new_op.make_node(*(list(fwd.inputs) + [_one_value(g) for g in gs]))
+        if new.outputs[-1].type != node.outputs[0].type:
+            continue
+        dx = node.outputs[0]
+        fgraph.replace(dx, new.outputs[-1])
+        for o, no in zip(fwd.outputs, new.outputs):
+            fgraph.replace(o, no)
+        count += 1
+    return count
 
 
 LIFT = {L.LayerNormalization: lambda op: HipLayerNormalization(op.epsilon),

@@ -868,6 +868,8 @@ def optimize(fgraph, fuse=True, rowchain=True, inplace=True):
     fgraph = lift_to_hip(fgraph)
     gof.merge_identical(fgraph)
     if fuse:
+        if hip_nnet.fuse_known_gradients(fgraph):
+            gof.merge_identical(fgraph)
         fuse_elemwise(fgraph)
         if rowchain:
             from .rowchain import fuse_row_chains

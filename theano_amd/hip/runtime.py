@@ -95,6 +95,8 @@ def _load():
         "thx_topk_distill_workspace": ([A, P(sz)], ctypes.c_int),
         "thx_topk_distill_call": ([A] * 3 + [ctypes.c_double, A, A, vp, sz, ctypes.c_int], ctypes.c_int),
         "thx_topk_distill_grad_call": ([A] * 5 + [ctypes.c_double, A, ctypes.c_int], ctypes.c_int),
+        "thx_token_logprob_train_call": ([A] * 4 + [ctypes.c_double] + [A] * 4 + [vp, sz, ctypes.c_int], ctypes.c_int),
+        "thx_topk_distill_train_call": ([A] * 4 + [ctypes.c_double] + [A] * 3 + [vp, sz, ctypes.c_int], ctypes.c_int),
         "thx_scratch_reserve": ([sz], ctypes.c_int),
         "thx_scratch_state": ([P(i64), P(i64), P(i64)], ctypes.c_int),
     }
