@@ -1,13 +1,9 @@
 // Layer normalisation over rows and its gradients: planner and kernels.
 #include "thx_rows.h"
-
-#include "kernels/thx_common.h"
+#include "thx_rows_device.h"
 
 namespace thx {
 namespace {
-
-template <class T> struct AccOf { typedef float type; };
-template <> struct AccOf<double> { typedef double type; };
 
 // ---- rows held in registers ----------------------------------------------------------------------------------------
 //
@@ -15,9 +11,9 @@ template <> struct AccOf<double> { typedef double type; };
 // around the mean and the result come out of registers.  Up to 64 threads of one wave need nothing but shuffles; larger
 // groups are whole blocks and pass the sums of their waves through LDS.
 
-template <class T> struct Width { enum { value = 16 / (int)sizeof(T) }; };
+template <int TPR> struct Block { enum { threads = TPR > 256 ? TPR : 256, rows = threads / TPR }; };
 
-// Sums of N values over the TPR threads of a row, in every one of them.  `lds`: N * TPR / 64 values per call, two sets of
+// Sums of N values over the TPR threads of a row, in every one of them.  `lds`: N values of every wave, two sets of
 // them used in turn, so that one barrier a call is enough: a set is written again two calls later, and by then every
 // wave has passed the barrier of the call between, behind its reads.
 template <int TPR, int N, class A>
@@ -28,11 +24,11 @@ THX_DEV void row_sums(A (&v)[N], A* lds, int& turn) {
     for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], m, 64);
   if constexpr (TPR > 64) {
     constexpr int W = TPR / 64;
-    A* set = lds + turn * N * W;
+    A* set = lds + (turn * Block<TPR>::rows + threadIdx.x / TPR) * N * W;
     turn ^= 1;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int k = 0; k < N; ++k) set[k * W + threadIdx.x / 64] = v[k];
+      for (int k = 0; k < N; ++k) set[k * W + threadIdx.x % TPR / 64] = v[k];
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < N; ++k) {
@@ -54,9 +50,9 @@ THX_DEV void load_edge(Vec<T, V>& v, const T* p, int64_t i, int64_t cols) {
   }
 }
 template <class T, int V>
-THX_DEV void store_edge(T* p, const Vec<T, V>& v, int64_t i, int64_t cols) {
+THX_DEV void store_edge(T* p, const Vec<T, V>& v, int64_t i, int64_t cols, bool nt) {
   if ((i + 1) * V <= cols) {
-    store_vec<T, V, false, true>(p + i * V, v);
+    store_out(p + i * V, v, nt);
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e)
@@ -67,32 +63,55 @@ THX_DEV void store_edge(T* p, const Vec<T, V>& v, int64_t i, int64_t cols) {
 THX_DEV float rsqrt_of(float v) { return 1.0f / sqrtf(v); }
 THX_DEV double rsqrt_of(double v) { return 1.0 / sqrt(v); }
 
-template <int TPR> struct Block { enum { threads = TPR > 256 ? TPR : 256, rows = threads / TPR }; };
+// A thread with at most 16 columns keeps their parameters in registers over all the rows its block goes through, and
+// loads the next row's vectors before it works on this one's.  Read anew for each row, single-precision parameters are
+// twice the traffic of a half-precision row (16384 rows of 4096 halves: 60 us, and 53 with this).
+template <class T, int VPT> struct Keep { enum { value = Width<T>::value * VPT <= 16 }; };
 
 template <class T, class P, int TPR, int VPT>
 __global__ void __launch_bounds__(Block<TPR>::threads) ln_forward(const T* x, int64_t xs, int64_t rows, int64_t cols,
                                                                   const P* gamma, const P* beta, double eps, T* y,
                                                                   typename AccOf<T>::type* mean,
-                                                                  typename AccOf<T>::type* invstd) {
+                                                                  typename AccOf<T>::type* invstd, bool nt) {
   typedef typename AccOf<T>::type A;
   constexpr int V = Width<T>::value, RPB = Block<TPR>::rows;
-  __shared__ A lds[TPR > 64 ? 2 * TPR / 64 : 1];
+  constexpr bool KEEP = Keep<T, VPT>::value;
+  __shared__ A lds[TPR > 64 ? 2 * Block<TPR>::threads / 64 : 1];
   const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
-  const A n = (A)cols;
+  const A share = (A)1 / (A)cols;
   int turn = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
-    const int64_t r = r0 + group < rows ? r0 + group : rows - 1;  // threads without a row repeat the last one
-    const T* xr = x + r * xs;
-    Vec<T, V> v[VPT];
+  // threads without a row repeat the last one
+  auto row_at = [&](int64_t r0) { return r0 + group < rows ? r0 + group : rows - 1; };
+  Vec<T, V> v[VPT], next[KEEP ? VPT : 1];
+  Vec<P, V> g[KEEP ? VPT : 1], b[KEEP ? VPT : 1];
+  if constexpr (KEEP) {
 #pragma unroll
-    for (int u = 0; u < VPT; ++u) load_edge(v[u], xr, u * TPR + t, cols);
+    for (int u = 0; u < VPT; ++u) {
+      load_edge(next[u], x + row_at((int64_t)blockIdx.x * RPB) * xs, u * TPR + t, cols);
+      if (gamma) load_edge(g[u], gamma, u * TPR + t, cols);
+      if (beta) load_edge(b[u], beta, u * TPR + t, cols);
+    }
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t r = row_at(r0);
+    const int64_t rn = row_at(r0 + (int64_t)gridDim.x * RPB);
+    const bool more = r0 + (int64_t)gridDim.x * RPB < rows;
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      if constexpr (KEEP) {
+        v[u] = next[u];
+        if (more) load_edge(next[u], x + rn * xs, u * TPR + t, cols);
+      } else {
+        load_edge(v[u], x + r * xs, u * TPR + t, cols);
+      }
+    }
     A sum[1] = {0};
 #pragma unroll
     for (int u = 0; u < VPT; ++u)
 #pragma unroll
       for (int e = 0; e < V; ++e) sum[0] += (A)v[u].v[e];
     row_sums<TPR>(sum, lds, turn);
-    const A mu = sum[0] / n;
+    const A mu = sum[0] * share;
     A sq[1] = {0};
 #pragma unroll
     for (int u = 0; u < VPT; ++u) {
@@ -104,24 +123,26 @@ __global__ void __launch_bounds__(Block<TPR>::threads) ln_forward(const T* x, in
       }
     }
     row_sums<TPR>(sq, lds, turn);
-    const A inv = rsqrt_of(sq[0] / n + (A)eps);
+    const A inv = rsqrt_of(sq[0] * share + (A)eps);
     T* yr = y + r * cols;
 #pragma unroll
     for (int u = 0; u < VPT; ++u) {
       const int64_t i = u * TPR + t;
+      const int w = KEEP ? u : 0;
       if (i * V >= cols) continue;
-      Vec<P, V> g, b;
-      if (gamma) load_edge(g, gamma, i, cols);
-      if (beta) load_edge(b, beta, i, cols);
+      if constexpr (!KEEP) {
+        if (gamma) load_edge(g[0], gamma, i, cols);
+        if (beta) load_edge(b[0], beta, i, cols);
+      }
       Vec<T, V> o;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        A w = ((A)v[u].v[e] - mu) * inv;
-        if (gamma) w *= (A)g.v[e];
-        if (beta) w += (A)b.v[e];
-        o.v[e] = (T)w;
+        A z = ((A)v[u].v[e] - mu) * inv;
+        if (gamma) z *= (A)g[w].v[e];
+        if (beta) z += (A)b[w].v[e];
+        o.v[e] = (T)z;
       }
-      store_edge(yr, o, i, cols);
+      store_edge(yr, o, i, cols, nt);
     }
     if (t == 0) mean[r] = mu, invstd[r] = inv;
   }
@@ -135,34 +156,48 @@ __global__ void __launch_bounds__(Block<TPR>::threads) ln_backward(const T* x, i
                                                                    int64_t rows, int64_t cols, const P* gamma,
                                                                    const typename AccOf<T>::type* mean, int64_t ms,
                                                                    const typename AccOf<T>::type* invstd, int64_t is, T* dx,
-                                                                   typename AccOf<T>::type* partial) {
+                                                                   typename AccOf<T>::type* partial, bool nt) {
   typedef typename AccOf<T>::type A;
   constexpr int V = Width<T>::value, RPB = Block<TPR>::rows;
-  __shared__ A lds[TPR > 64 ? 4 * TPR / 64 : 1];
+  __shared__ A lds[TPR > 64 ? 4 * Block<TPR>::threads / 64 : 1];
   const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
-  const A n = (A)cols;
+  const A share = (A)1 / (A)cols;
   int turn = 0;
   A dg[PARAMS ? VPT : 1][V], db[PARAMS ? VPT : 1][V];
 #pragma unroll
   for (int u = 0; u < (PARAMS ? VPT : 1); ++u)
 #pragma unroll
     for (int e = 0; e < V; ++e) dg[u][e] = db[u][e] = 0;
+  // the next row's vectors are on their way while this one's are worked on, where registers are left for them
+  constexpr bool AHEAD = TPR < 1024 || V * VPT < 16;
+  auto row_at = [&](int64_t r0) { return r0 + group < rows ? r0 + group : rows - 1; };
+  Vec<T, V> v[VPT], d[VPT], vn[VPT], dn[VPT];
+  Vec<P, V> g[VPT];
+  A mn = 0, in = 0;
+  auto load = [&](int64_t r) {
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      load_edge(vn[u], x + r * xs, u * TPR + t, cols);
+      load_edge(dn[u], dy + r * ds, u * TPR + t, cols);  // 0 behind the end: those columns add nothing
+    }
+    mn = mean[r * ms];
+    in = invstd[r * is];
+  };
+  if (AHEAD && (int64_t)blockIdx.x * RPB < rows) load(row_at((int64_t)blockIdx.x * RPB));
+#pragma unroll
+  for (int u = 0; u < VPT; ++u)
+    if (gamma) load_edge(g[u], gamma, u * TPR + t, cols);
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
     const bool live = r0 + group < rows;
-    const int64_t r = live ? r0 + group : rows - 1;
-    const T *xr = x + r * xs, *dr = dy + r * ds;
-    Vec<T, V> v[VPT], d[VPT];
+    const int64_t r = row_at(r0);
+    if (!AHEAD) load(r);
+    const A mu = mn, inv = in;
 #pragma unroll
-    for (int u = 0; u < VPT; ++u) {
-      load_edge(v[u], xr, u * TPR + t, cols);
-      load_edge(d[u], dr, u * TPR + t, cols);  // 0 behind the end: those columns add nothing
-    }
-    const A mu = mean[r * ms], inv = invstd[r * is];
+    for (int u = 0; u < VPT; ++u) v[u] = vn[u], d[u] = dn[u];
+    if (AHEAD && r0 + (int64_t)gridDim.x * RPB < rows) load(row_at(r0 + (int64_t)gridDim.x * RPB));
     A s[2] = {0, 0};
-    Vec<P, V> g[VPT];
 #pragma unroll
     for (int u = 0; u < VPT; ++u) {
-      if (gamma) load_edge(g[u], gamma, u * TPR + t, cols);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const A dv = (A)d[u].v[e], a = gamma ? dv * (A)g[u].v[e] : dv, xh = ((A)v[u].v[e] - mu) * inv;
@@ -175,8 +210,8 @@ __global__ void __launch_bounds__(Block<TPR>::threads) ln_backward(const T* x, i
       }
     }
     row_sums<TPR>(s, lds, turn);
-    s[0] /= n;
-    s[1] /= n;
+    s[0] *= share;
+    s[1] *= share;
     T* out = dx + r * cols;
 #pragma unroll
     for (int u = 0; u < VPT; ++u) {
@@ -188,7 +223,7 @@ __global__ void __launch_bounds__(Block<TPR>::threads) ln_backward(const T* x, i
         const A dv = (A)d[u].v[e], a = gamma ? dv * (A)g[u].v[e] : dv, xh = ((A)v[u].v[e] - mu) * inv;
         o.v[e] = (T)(inv * (a - s[0] - xh * s[1]));
       }
-      store_edge(out, o, i, cols);
+      store_edge(out, o, i, cols, nt);
     }
   }
   if constexpr (PARAMS) {
@@ -373,31 +408,42 @@ struct Shape {
   int tpr = 0, vpt = 0;
 };
 
-// The smallest group of threads that holds a row in registers.  Forward: up to 8 vectors to a thread, so that rows of up to
-// 4096 halves stay within one wave and need no barrier.  Backward a thread keeps two more sums per column, so a quarter of
-// the columns, and longer rows take whole blocks.
+// The smallest group of threads that holds a row in registers; tpr 0 where none does or a parameter's values do not lie
+// side by side.  Forward 16 columns to a thread, with their parameters kept: rows of 4096 halves as 256 threads x 2
+// vectors 53 us, 64 x 8 87 us (parameters read for every row), rows of 1024 floats 64 x 4 48 us, 256 x 1 53 us.  Backward
+// a thread keeps two sums more per column: rows of 1024 floats 128 x 2 78 us, 64 x 4 81 us, of 8192 halves 1024 x 1 87 us,
+// 512 x 2 101 us.
 Shape shape_of(int64_t cols, int dtype, bool backward, bool packed) {
-  const int64_t nv = (cols * dtype_size(dtype) + 15) / 16;
-  static const Shape forward[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {64, 8}, {256, 4}, {256, 8}, {1024, 8}};
-  static const Shape back[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {1024, 1}, {1024, 2}};
-  Shape none;
-  if (!packed || !cols) return none;
-  if (backward) {
-    for (const Shape& s : back)
-      if (nv <= (int64_t)s.tpr * s.vpt) return s;
-  } else {
-    for (const Shape& s : forward)
-      if (nv <= (int64_t)s.tpr * s.vpt) return s;
-  }
-  return none;
+  static const Shape halves[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {128, 2}, {256, 2}, {512, 2}, {1024, 2}, {1024, 4}, {1024, 8}};
+  static const Shape words[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {128, 4}, {256, 4}, {512, 4}, {1024, 4}, {1024, 8}};
+  static const Shape back[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {128, 2}, {256, 2}, {1024, 1}, {1024, 2}};
+  const int isz = dtype_size(dtype);
+  const int64_t vectors = (cols * isz + 15) / 16;
+  auto first = [&](const Shape* s, int n) {
+    for (int k = 0; k < n; ++k)
+      if (vectors <= (int64_t)s[k].tpr * s[k].vpt) return s[k];
+    return Shape();
+  };
+  if (!packed || !cols) return Shape();
+  return backward ? first(back, 9) : isz == 2 ? first(halves, 11) : first(words, 11);
 }
 
-// Blocks of the gradients' pass: as many as the device runs at once, no more than there are rows for.  Each leaves one
-// set of sums, so more of them would only be more to add up.
+// Blocks for rows in groups of as many as a block takes at once: at most `most`, each with the same number of turns.
+int64_t even_blocks(const Shape& s, int64_t rows, int64_t most) {
+  const int64_t per = s.tpr > 256 ? 1 : 256 / s.tpr, groups = (rows + per - 1) / per;
+  const int64_t turns = std::max<int64_t>(1, (groups + most - 1) / most);
+  return std::max<int64_t>(1, (groups + turns - 1) / turns);
+}
+
+// As many threads as the device holds.
+int64_t forward_blocks(const Shape& s, int64_t rows) {
+  return even_blocks(s, rows, (int64_t)compute_units() * (2048 / std::max(256, s.tpr)));
+}
+
+// Every block leaves one set of sums for ln_join, so no more of them than it takes to keep the memory busy: rows of 4096
+// halves, 256 x 2, with 1, 2 and 4 blocks to a compute unit 133, 89 and 108 us; rows of 512, 64 x 1, 185, 113 and 84.
 int64_t backward_blocks(const Shape& s, int64_t rows) {
-  const int64_t per = s.tpr > 256 ? 1 : 256 / s.tpr;
-  const int64_t most = (int64_t)compute_units() * (s.tpr > 256 ? 1 : 4);
-  return std::max<int64_t>(1, std::min<int64_t>(most, (rows + per - 1) / per));
+  return even_blocks(s, rows, (int64_t)compute_units() * (s.tpr > 256 ? 1 : s.vpt > 1 ? 2 : 4));
 }
 
 int slices_of(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>(64, rows / 64)); }
@@ -405,7 +451,23 @@ int slices_of(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>
 // f(integral constants TPR, VPT) for a shape.
 template <int TPR, int VPT> struct Held { enum { tpr = TPR, vpt = VPT }; };
 template <class F>
-int by_shape(const Shape& s, F&& f) {
+int by_shape_halves(const Shape& s, F&& f) {
+  switch (s.tpr * 16 + s.vpt) {
+    case 8 * 16 + 1: return f(Held<8, 1>());
+    case 16 * 16 + 1: return f(Held<16, 1>());
+    case 32 * 16 + 1: return f(Held<32, 1>());
+    case 64 * 16 + 1: return f(Held<64, 1>());
+    case 64 * 16 + 2: return f(Held<64, 2>());
+    case 128 * 16 + 2: return f(Held<128, 2>());
+    case 256 * 16 + 2: return f(Held<256, 2>());
+    case 512 * 16 + 2: return f(Held<512, 2>());
+    case 1024 * 16 + 2: return f(Held<1024, 2>());
+    case 1024 * 16 + 4: return f(Held<1024, 4>());
+    default: return f(Held<1024, 8>());
+  }
+}
+template <class F>
+int by_shape_words(const Shape& s, F&& f) {
   switch (s.tpr * 16 + s.vpt) {
     case 8 * 16 + 1: return f(Held<8, 1>());
     case 16 * 16 + 1: return f(Held<16, 1>());
@@ -413,11 +475,17 @@ int by_shape(const Shape& s, F&& f) {
     case 64 * 16 + 1: return f(Held<64, 1>());
     case 64 * 16 + 2: return f(Held<64, 2>());
     case 64 * 16 + 4: return f(Held<64, 4>());
-    case 64 * 16 + 8: return f(Held<64, 8>());
+    case 128 * 16 + 4: return f(Held<128, 4>());
     case 256 * 16 + 4: return f(Held<256, 4>());
-    case 256 * 16 + 8: return f(Held<256, 8>());
+    case 512 * 16 + 4: return f(Held<512, 4>());
+    case 1024 * 16 + 4: return f(Held<1024, 4>());
     default: return f(Held<1024, 8>());
   }
+}
+template <class T, class F>
+int by_shape(const Shape& s, F&& f) {
+  if constexpr (sizeof(T) == 2) return by_shape_halves(s, f);
+  else return by_shape_words(s, f);
 }
 template <class F>
 int by_back_shape(const Shape& s, F&& f) {
@@ -427,7 +495,7 @@ int by_back_shape(const Shape& s, F&& f) {
     case 32 * 16 + 1: return f(Held<32, 1>());
     case 64 * 16 + 1: return f(Held<64, 1>());
     case 64 * 16 + 2: return f(Held<64, 2>());
-    case 256 * 16 + 1: return f(Held<256, 1>());
+    case 128 * 16 + 2: return f(Held<128, 2>());
     case 256 * 16 + 2: return f(Held<256, 2>());
     case 1024 * 16 + 1: return f(Held<1024, 1>());
     default: return f(Held<1024, 2>());
@@ -472,6 +540,7 @@ int layernorm(const thx_array* x, const thx_array* gamma, const thx_array* beta,
   set_last_plan(plan);
   if (dry || !in[0].rows) return THX_OK;
   if ((rc = ensure_init())) return rc;
+  bool nt = stream_out(in[0], out[0]);
   return by_types(in[0].dtype, pt, [&](auto t, auto p) {
     typedef decltype(t) T;
     typedef decltype(p) P;
@@ -480,13 +549,12 @@ int layernorm(const thx_array* x, const thx_array* gamma, const thx_array* beta,
                       &in[2].stride, &epsilon, &out[0].ptr, &out[1].ptr, &out[2].ptr};
       return launch_builtin((const void*)&ln_forward_any<T, P>, plan, dim3(grid_of(in[0].rows)), dim3(1024), args);
     }
-    return by_shape(shape, [&](auto h) {
+    return by_shape<T>(shape, [&](auto h) {
       constexpr int TPR = decltype(h)::tpr, VPT = decltype(h)::vpt;
       void* args[] = {&in[0].ptr, &in[0].stride, &in[0].rows, &in[0].cols, &in[1].ptr, &in[2].ptr, &epsilon, &out[0].ptr,
-                      &out[1].ptr, &out[2].ptr};
-      const int64_t per = Block<TPR>::rows;
-      return launch_builtin((const void*)&ln_forward<T, P, TPR, VPT>, plan, dim3(grid_of((in[0].rows + per - 1) / per)),
-                            dim3(Block<TPR>::threads), args);
+                      &out[1].ptr, &out[2].ptr, &nt};
+      return launch_builtin((const void*)&ln_forward<T, P, TPR, VPT>, plan,
+                            dim3(grid_of(forward_blocks(shape, in[0].rows))), dim3(Block<TPR>::threads), args);
     });
   });
 }
@@ -540,6 +608,7 @@ int layernorm_grad(const thx_array* x, const thx_array* dy, const thx_array* gam
   set_last_plan(plan);
   if (dry || !in[0].cols) return THX_OK;
   if ((rc = ensure_init())) return rc;
+  bool nt = stream_out(in[0], out[0]);
   return by_types(in[0].dtype, pt, [&](auto t, auto p) {
     typedef decltype(t) T;
     typedef decltype(p) P;
@@ -551,7 +620,7 @@ int layernorm_grad(const thx_array* x, const thx_array* dy, const thx_array* gam
       rc = by_back_shape(shape, [&](auto h) {
         constexpr int TPR = decltype(h)::tpr, VPT = decltype(h)::vpt;
         void* args[] = {&in[0].ptr, &in[0].stride, &in[1].ptr, &in[1].stride, &in[0].rows, &in[0].cols, &in[4].ptr,
-                        &in[2].ptr, &in[2].stride, &in[3].ptr, &in[3].stride, &out[0].ptr, &ws};
+                        &in[2].ptr, &in[2].stride, &in[3].ptr, &in[3].stride, &out[0].ptr, &ws, &nt};
         const void* kernel = dgamma ? (const void*)&ln_backward<T, P, TPR, VPT, true>
                                     : (const void*)&ln_backward<T, P, TPR, VPT, false>;
         return launch_builtin(kernel, plan, dim3(blocks), dim3(Block<TPR>::threads), args);

@@ -31,6 +31,7 @@ struct Rows {
   int dtype = 0, nd = 0;
   int64_t rows = 1, cols = 1;
   int64_t stride = 0;              // elements between rows
+  bool reused = false;             // THX_REUSED
   const char *lo = nullptr, *hi = nullptr;  // the bytes it spans, for the overlap check
 };
 
@@ -43,6 +44,7 @@ inline int rows_of(const char* what, const char* name, const thx_array* a, int d
   if (a->dtype & (THX_HOST_SCALAR | THX_INDEX))
     return fail(THX_ERR_TYPE, "%s: %s must be a device array", what, name);
   r->dtype = a->dtype & ~THX_REUSED;
+  r->reused = (a->dtype & THX_REUSED) != 0;
   const int isz = dtype_size(r->dtype);
   if (!isz || (dtype >= 0 && r->dtype != dtype))
     return fail(THX_ERR_TYPE, "%s: %s has dtype code %d, expected %d", what, name, r->dtype, dtype);
@@ -125,6 +127,13 @@ inline int check_workspace(const char* what, void* ws, size_t have, size_t need,
   if (need && !ws && !(flags & THX_DRY_RUN)) return fail(THX_ERR_ARG, "%s: the workspace has no address", what);
   if ((uintptr_t)ws % 16) return fail(THX_ERR_ARG, "%s: the workspace must be aligned to 16 bytes", what);
   return THX_OK;
+}
+
+// Whether a result as large as the rows `x` it comes from is written past the caches: where the two together exceed what
+// the last-level cache holds for a reader, unless the caller says that one follows.  Measured on gradients of 2048 rows
+// of 32000 floats 138 -> 125 us, of 4096 rows of 128000 halves 579 -> 555; below the border such stores are slower.
+inline bool stream_out(const Rows& x, const Rows& out) {
+  return !out.reused && nt_streaming(2 * x.rows * x.cols * dtype_size(x.dtype));
 }
 
 inline int compute_units() { return rt().cus ? rt().cus : 256; }

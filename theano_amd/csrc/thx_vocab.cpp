@@ -4,14 +4,10 @@
 // Everything is computed in binary logarithms: with c = log2(e) / temperature, s_j = c * x_j and the row's largest
 // logit m, S = sum_j 2^(s_j - c m), so log2 p_j = (s_j - c m) - log2 S.  A row keeps (m, log2 S).
 #include "thx_rows.h"
-
-#include "kernels/thx_common.h"
+#include "thx_rows_device.h"
 
 namespace thx {
 namespace {
-
-template <class T> struct AccOf { typedef float type; };
-template <> struct AccOf<double> { typedef double type; };
 
 constexpr double kLog2E = 1.44269504088896340735992468100189214;
 constexpr double kLn2 = 0.693147180559945309417232121458176568;
@@ -90,7 +86,6 @@ template <class Key> THX_DEV int64_t key_column(Key k) { return (int64_t)(0xffff
 constexpr int kUnroll = 4;
 constexpr int kWaves = 4;     // waves of a block; each works alone
 constexpr int kList = 512;    // candidates a wave can hold
-template <class T> struct Width { enum { value = 16 / (int)sizeof(T) }; };
 
 template <class T, bool ENT>
 struct LaneSums {
@@ -638,6 +633,7 @@ struct GradCut {
   int segs;     // segments of a row
   A c;
   T* dx;
+  bool nt;      // dx is streamed past the caches
 };
 
 
@@ -726,7 +722,7 @@ __global__ void __launch_bounds__(256) vocab_grad(GradCut<T> q, Row row) {
       for (int u = 0; u < kUnroll; ++u) {
         const int64_t i = i0 + u * 256 + threadIdx.x;
         if (i < hi && i < whole) {
-          store_vec<T, V, false, true>(dx + i * V, v[u]);
+          store_out(dx + i * V, v[u], q.nt);
         } else if (i < hi) {
           for (int64_t j = i * V; j < q.cols; ++j) dx[j] = slope.none ? (T)0 : (T)slope(x[j]);
         }
@@ -760,14 +756,6 @@ struct KdTrain {
   const A* g; int64_t gs;
   A temperature;
 };
-
-// The compiler forgets what it knows about a vector's values: without this it keeps single-precision copies of a row's
-// elements from the first use to the second, which is twice the registers.
-template <class T, int V>
-THX_DEV void forget(Vec<T, V>& v) {
-  thx_u32x4& raw = *(thx_u32x4*)&v;
-  asm volatile("" : "+v"(raw));
-}
 
 template <class T, class Row, int THREADS, int VPT>
 __global__ void __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 8 && sizeof(T) < 8 ? 8 : 1)
@@ -894,7 +882,7 @@ vocab_train(GradCut<T> q, Row row) {
       if (u > full) continue;
       Vec<T, V> o[1] = {v[u]};
       slope.over(o);
-      if (u < full || u * THREADS + (int)threadIdx.x < whole) store_vec<T, V, false, true>(dt + u * (THREADS * V), o[0]);
+      if (u < full || u * THREADS + (int)threadIdx.x < whole) store_out(dt + u * (THREADS * V), o[0], q.nt);
     }
     if (extra) dx[(int64_t)whole * V + threadIdx.x] = slope.none ? (T)0 : (T)slope(tail);
     __syncthreads();  // the entries and the losses are there, and the elements that the entries replace are written
@@ -967,7 +955,7 @@ int launch_forward(Cut<T> q, Row row, const std::string& plan) {
 // least; whole rows else, since every segment reads the row's list again (2048 rows of 32000 floats, 64 entries: 153 us
 // in segments of 4 vectors to a thread, 116 us in two segments a row).
 template <class T, class Row>
-int launch_grad(const Rows& x, double temperature, char* dx, Row row, const std::string& plan) {
+int launch_grad(const Rows& x, double temperature, const Rows& dx, Row row, const std::string& plan) {
   typedef typename AccOf<T>::type A;
   GradCut<T> q;
   const int64_t vectors = ceil_div(x.cols, Width<T>::value);
@@ -976,7 +964,8 @@ int launch_grad(const Rows& x, double temperature, char* dx, Row row, const std:
   q.segs = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(vectors, 256), ceil_div(16 * compute_units(), x.rows)));
   q.per = ceil_div(vectors, q.segs);
   q.c = (A)(kLog2E / temperature);
-  q.dx = (T*)dx;
+  q.dx = (T*)dx.ptr;
+  q.nt = stream_out(x, dx);
   void* args[] = {&q, &row};
   return launch_builtin((const void*)&vocab_grad<T, Row>, plan, dim3(grid_of(x.rows * q.segs)), dim3(256), args);
 }
@@ -999,13 +988,14 @@ std::string held_plan(const char* name, const Rows& x, const Hold& h) {
 }
 
 template <class T, class Row>
-int launch_train(const Rows& x, double temperature, char* dx, const Hold& h, Row row, const std::string& plan) {
+int launch_train(const Rows& x, double temperature, const Rows& dx, const Hold& h, Row row, const std::string& plan) {
   typedef typename AccOf<T>::type A;
   GradCut<T> q = {};
   q.x = (const T*)x.ptr;
   q.xs = x.stride, q.rows = x.rows, q.cols = x.cols;
   q.c = (A)(kLog2E / temperature);
-  q.dx = (T*)dx;
+  q.dx = (T*)dx.ptr;
+  q.nt = stream_out(x, dx);
   void* args[] = {&q, &row};
   const void* kernel = nullptr;
   switch (h.threads * 32 + h.vpt) {
@@ -1131,7 +1121,7 @@ int token_logprob_grad(const thx_array* logits, const thx_array* tokens, const t
     const LpGrad<A> q = {in[1].ptr, in[1].stride, in[1].dtype == THX_I64, (const A*)in[2].ptr, in[2].stride, (const A*)in[3].ptr,
                    in[3].stride, (const int64_t*)in[4].ptr, in[4].stride, (int)n_top, (const A*)in[5].ptr, in[5].stride,
                    (const A*)in[6].ptr, in[6].stride, (const A*)in[7].ptr, in[7].stride, (A)(1.0 / temperature)};
-    return launch_grad<T>(in[0], temperature, out.ptr, q, plan);
+    return launch_grad<T>(in[0], temperature, out, q, plan);
   });
 }
 
@@ -1206,7 +1196,7 @@ int topk_distill_grad(const thx_array* logits, const thx_array* teacher, const t
     typedef typename AccOf<T>::type A;
     const KdGrad<A> row = {teacher_args<A>(in[1], in[2]), (const A*)in[3].ptr, in[3].stride, (const A*)in[4].ptr,
                            in[4].stride, (A)(kLog2E / temperature), (A)temperature};
-    return launch_grad<T>(in[0], temperature, out.ptr, row, plan);
+    return launch_grad<T>(in[0], temperature, out, row, plan);
   });
 }
 
@@ -1246,7 +1236,7 @@ int token_logprob_train(const thx_array* logits, const thx_array* tokens, const 
     const LpTrain<T> row = {{t.ptr, t.stride, t.dtype == THX_I64, 0, (A)(1.0 / temperature),
                              {(A*)out[0].ptr, (A*)out[1].ptr, nullptr, nullptr, (A*)out[2].ptr}},
                             (const A*)gr.ptr, gr.stride, (const A*)ur.ptr, ur.stride};
-    return launch_train<T>(x, temperature, out[3].ptr, h, row, plan);
+    return launch_train<T>(x, temperature, out[3], h, row, plan);
   });
 }
 
@@ -1282,7 +1272,7 @@ int topk_distill_train(const thx_array* logits, const thx_array* teacher, const 
     const KdTrain<T> row = {{teacher_args<A>(t, ids), (A)(1.0 / temperature), (A)(temperature * temperature),
                              (A*)out[0].ptr, (A*)out[1].ptr},
                             (const A*)gr.ptr, gr.stride, (A)temperature};
-    return launch_train<T>(x, temperature, out[2].ptr, h, row, plan);
+    return launch_train<T>(x, temperature, out[2], h, row, plan);
   });
 }
 
