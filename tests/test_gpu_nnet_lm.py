@@ -763,7 +763,7 @@ def test_views_of_and_for_other_libraries():
     v = rng.standard_normal((6, 40)).astype("float32")
     a = HipArray.from_numpy(v)
     d = a.__cuda_array_interface__
-    assert d["shape"] == (6, 40) and d["typestr"] == "<f4" and d["strides"] is None and d["data"] == (a.ptr, False)
+    assert d["shape"] == (6, 40) and d["typestr"] == "<f4" and d["strides"] == (160, 4) and d["data"] == (a.ptr, False)
     assert d["stream"] == hip.stream() and d["stream"]
     b = HipArray.from_cuda_array_interface(Other(a))
     assert b.ptr == a.ptr and b.shape == a.shape and b.strides == a.strides and b.dtype == a.dtype

@@ -15,13 +15,15 @@ from ..tensor import nnet_lm as L
 from ..tensor.elemwise import DimShuffle, Elemwise
 from ..tensor.type import TensorType
 from .ops import HipArrayType, as_hip_variable
-from .runtime import HipArray, _Buffer, call_flags, check, lib, mark_reused, thx_array
+from .runtime import HipArray, _Buffer, _CODE_OF, _c_strides, call_flags, check, lib, mark_reused, thx_array
 
 _UNSUPPORTED = 6
 
 
 class _RowOp(object):
-    """``make_node`` and the calling sequence shared by the operators."""
+    """``make_node`` and the calling sequence shared by the operators; ``call(node, ins, outs)`` gives the library
+    function, its arguments up to the workspace, and the query for the workspace's size with its arguments (None where
+    the function takes no workspace)."""
 
     def make_node(self, *inputs):
         ins = [as_hip_variable(i) for i in inputs]
@@ -31,46 +33,92 @@ class _RowOp(object):
         return Apply(self, ins, [HipArrayType(o.type.dtype, o.type.broadcastable)() for o in host.outputs])
 
     def perform(self, node, inputs, output_storage):
-        slots = node.tag.get("thx")
-        if slots is None:
-            slots = node.tag["thx"] = ((thx_array * len(inputs))(), (thx_array * len(node.outputs))(),
-                                       [np.dtype(o.type.dtype) for o in node.outputs])
-        ins, outs, dtypes = slots
-        shapes = self.infer_shape(node, [i.shape for i in inputs])
-        results = []
-        for k, v in enumerate(inputs):
-            v.as_thx(ins[k])
-        for k, dt in enumerate(dtypes):
-            arr = HipArray._new_contiguous(tuple(shapes[k]), dt)
-            arr.as_thx(outs[k])
-            results.append(arr)
-        mark_reused(node, ins, outs)
-        flags = call_flags(node)
-        rc = self.call(node, ins, outs, flags)
-        if rc == _UNSUPPORTED:          # rows at more than one stride, or columns apart
-            copies = [v if v.c_contiguous else v.copy() for v in inputs]
-            if all(c is v for c, v in zip(copies, inputs)):
-                check(rc)
-            for k, v in enumerate(copies):
-                v.as_thx(ins[k])
-            rc = self.call(node, ins, outs, flags)
-        if rc:
-            check(rc)
+        state = node.tag.get("thx")
+        if state is None:
+            state = node.tag["thx"] = _State(self, node)
+        results = state.run(inputs, call_flags(node))
         for k, arr in enumerate(results):
             output_storage[k][0] = arr
 
-    def workspace(self, node, ins, query, *args):
-        """A buffer for the partial results of a call on ``ins``, kept for the length of the call alone (or by the
-        recording the call is made in): (address, size)."""
-        key = (tuple(ins[0].shape[:ins[0].nd]),) + tuple(ins[0].strides_bytes[:ins[0].nd])
-        known = node.tag.get("workspace")
-        if known is None or known[0] != key:
+
+class _State(object):
+    """What a node keeps from one call to the next: the descriptors of its operands and results, the library call's
+    arguments (addresses of those descriptors), and for the layout of the last call the results' shapes, the offsets of
+    the small ones in a buffer they share, and the size of the workspace.  No values and no addresses of data."""
+
+    _SHARED = 1 << 16      # results of up to so many bytes lie in one buffer with others of the same call
+
+    def __init__(self, op, node):
+        self.op, self.node = op, node
+        self.ins = (thx_array * len(node.inputs))()
+        self.outs = (thx_array * len(node.outputs))()
+        self.in_slots, self.out_slots = list(self.ins), list(self.outs)
+        self.dtypes = [np.dtype(o.type.dtype) for o in node.outputs]
+        self.fn, self.args, self.query = op.call(node, self.ins, self.outs)
+        self.layout = None
+
+    def plan(self, inputs, layout):
+        """Everything of a call that depends on the operands' layout alone."""
+        self.layout = None
+        for v, slot in zip(inputs, self.in_slots):
+            v.as_thx(slot)
+        shapes = [tuple(s) for s in self.op.infer_shape(self.node, [v.shape for v in inputs])]
+        self.results, at, together = [], 0, []
+        for k, (shape, dtype) in enumerate(zip(shapes, self.dtypes)):
+            nbytes = dtype.itemsize
+            for s in shape:
+                nbytes *= s
+            if nbytes <= self._SHARED:
+                together.append(k)
+                offset, at = at, at + (nbytes + 63) // 64 * 64
+            else:
+                offset = None
+            self.results.append((shape, _c_strides(shape, dtype.itemsize), dtype, _CODE_OF[dtype], nbytes, offset))
+        self.shared_bytes = at
+        for (shape, strides, dtype, code, nbytes, offset), slot in zip(self.results, self.out_slots):
+            slot.offset_bytes, slot.nd, slot.dtype = offset or 0, len(shape), code
+            slot.shape[:len(shape)] = shape
+            slot.strides_bytes[:len(shape)] = strides
+        mark_reused(self.node, self.ins, self.outs)
+        self.workspace = 0
+        if self.query is not None:
             n = ctypes.c_size_t()
-            rc = query(ctypes.byref(ins[0]), *(args + (ctypes.byref(n),)))
+            rc = self.query[0](*(self.query[1:] + (ctypes.byref(n),)))
             if rc:
-                return rc, None, 0
-            known = node.tag["workspace"] = (key, n.value)
-        return 0, (_Buffer(known[1]) if known[1] else None), known[1]
+                return rc
+            self.workspace = n.value
+        self.layout = layout
+        return 0
+
+    def run(self, inputs, flags):
+        layout = [(v.shape, v.strides) for v in inputs]
+        rc = 0
+        if layout != self.layout:
+            rc = self.plan(inputs, layout)
+        else:
+            for v, slot in zip(inputs, self.in_slots):
+                slot.base = v.buffer.ptr
+                slot.offset_bytes = v.offset
+        if not rc:
+            shared = _Buffer(self.shared_bytes) if self.shared_bytes else None
+            results = []
+            for (shape, strides, dtype, code, nbytes, offset), slot in zip(self.results, self.out_slots):
+                buffer = _Buffer(nbytes) if offset is None else shared
+                slot.base = buffer.ptr
+                results.append(HipArray._raw(buffer, offset or 0, shape, strides, dtype, code))
+            if self.query is None:
+                rc = self.fn(*self.args, flags)
+            else:
+                # kept for the length of the call alone, or by the recording the call is made in
+                ws = _Buffer(self.workspace) if self.workspace else None
+                rc = self.fn(*self.args, ws.ptr if ws else None, self.workspace, flags)
+            if not rc:
+                return results
+        if rc == _UNSUPPORTED:          # rows at more than one stride, or columns apart
+            copies = [v if v.c_contiguous else v.copy() for v in inputs]
+            if any(c is not v for c, v in zip(copies, inputs)):
+                return self.run(copies, flags)
+        check(rc)
 
 
 def _at(arrays, k):
@@ -80,60 +128,59 @@ def _at(arrays, k):
 class HipLayerNormalization(_RowOp, L.LayerNormalization):
     host_op = L.LayerNormalization
 
-    def call(self, node, ins, outs, flags):
+    def call(self, node, ins, outs):
         n = len(node.inputs)
-        return lib.thx_layernorm_call(_at(ins, 0), _at(ins, 1 if n > 1 else None), _at(ins, 2 if n > 2 else None),
-                                      self.epsilon, _at(outs, 0), _at(outs, 1), _at(outs, 2), flags)
+        return lib.thx_layernorm_call, (_at(ins, 0), _at(ins, 1 if n > 1 else None), _at(ins, 2 if n > 2 else None),
+                                        self.epsilon, _at(outs, 0), _at(outs, 1), _at(outs, 2)), None
 
 
 class HipLayerNormalizationGrad(_RowOp, L.LayerNormalizationGrad):
     host_op = L.LayerNormalizationGrad
 
-    def call(self, node, ins, outs, flags):
+    def call(self, node, ins, outs):
         n = self.n_params
-        rc, ws, size = self.workspace(node, ins, lib.thx_layernorm_grad_workspace, _at(outs, 1 if n else None))
-        return rc or lib.thx_layernorm_grad_call(
-            _at(ins, 0), _at(ins, 1), _at(ins, 4 if n else None), _at(ins, 2), _at(ins, 3), _at(outs, 0),
-            _at(outs, 1 if n else None), _at(outs, 2 if n > 1 else None), ws.ptr if ws else None, size, flags)
+        dgamma = _at(outs, 1 if n else None)
+        return lib.thx_layernorm_grad_call, (
+            _at(ins, 0), _at(ins, 1), _at(ins, 4 if n else None), _at(ins, 2), _at(ins, 3), _at(outs, 0), dgamma,
+            _at(outs, 2 if n > 1 else None)), (lib.thx_layernorm_grad_workspace, _at(ins, 0), dgamma)
 
 
 class HipTokenLogProbs(_RowOp, L.TokenLogProbs):
     host_op = L.TokenLogProbs
 
-    def call(self, node, ins, outs, flags):
-        rc, ws, size = self.workspace(node, ins, lib.thx_token_logprob_workspace, self.n_top)
+    def call(self, node, ins, outs):
         k = self.n_top
-        return rc or lib.thx_token_logprob_call(
+        return lib.thx_token_logprob_call, (
             _at(ins, 0), _at(ins, 1), self.temperature, k, _at(outs, 0), _at(outs, 1), _at(outs, 2 if k else None),
-            _at(outs, 3 if k else None), _at(outs, 4 if k else 2), ws.ptr if ws else None, size, flags)
+            _at(outs, 3 if k else None), _at(outs, 4 if k else 2)), (lib.thx_token_logprob_workspace, _at(ins, 0), k)
 
 
 class HipTokenLogProbsGrad(_RowOp, L.TokenLogProbsGrad):
     host_op = L.TokenLogProbsGrad
 
-    def call(self, node, ins, outs, flags):
+    def call(self, node, ins, outs):
         at = iter(range(4, len(node.inputs)))
         top = next(at) if self.given[2] else None
         g, u, gt = [next(at) if there else None for there in self.given]
-        return lib.thx_token_logprob_grad_call(_at(ins, 0), _at(ins, 1), _at(ins, 2), _at(ins, 3), _at(ins, top), _at(ins, g),
-                                               _at(ins, u), _at(ins, gt), self.temperature, _at(outs, 0), flags)
+        return lib.thx_token_logprob_grad_call, (_at(ins, 0), _at(ins, 1), _at(ins, 2), _at(ins, 3), _at(ins, top),
+                                                 _at(ins, g), _at(ins, u), _at(ins, gt), self.temperature,
+                                                 _at(outs, 0)), None
 
 
 class HipTopKDistillation(_RowOp, L.TopKDistillation):
     host_op = L.TopKDistillation
 
-    def call(self, node, ins, outs, flags):
-        rc, ws, size = self.workspace(node, ins, lib.thx_topk_distill_workspace)
-        return rc or lib.thx_topk_distill_call(_at(ins, 0), _at(ins, 1), _at(ins, 2), self.temperature, _at(outs, 0),
-                                               _at(outs, 1), ws.ptr if ws else None, size, flags)
+    def call(self, node, ins, outs):
+        return lib.thx_topk_distill_call, (_at(ins, 0), _at(ins, 1), _at(ins, 2), self.temperature, _at(outs, 0),
+                                           _at(outs, 1)), (lib.thx_topk_distill_workspace, _at(ins, 0))
 
 
 class HipTopKDistillationGrad(_RowOp, L.TopKDistillationGrad):
     host_op = L.TopKDistillationGrad
 
-    def call(self, node, ins, outs, flags):
-        return lib.thx_topk_distill_grad_call(_at(ins, 0), _at(ins, 1), _at(ins, 2), _at(ins, 3), _at(ins, 4),
-                                              self.temperature, _at(outs, 0), flags)
+    def call(self, node, ins, outs):
+        return lib.thx_topk_distill_grad_call, (_at(ins, 0), _at(ins, 1), _at(ins, 2), _at(ins, 3), _at(ins, 4),
+                                                self.temperature, _at(outs, 0)), None
 
 
 class _TrainOp(_RowOp):
@@ -165,13 +212,12 @@ class HipTokenLogProbsTrain(_TrainOp, Op):
         self.temperature, self.given = float(temperature), tuple(bool(g) for g in given)
         self.forward = HipTokenLogProbs(0, temperature)
 
-    def call(self, node, ins, outs, flags):
-        rc, ws, size = self.workspace(node, ins, lib.thx_token_logprob_workspace, 0)
+    def call(self, node, ins, outs):
         at = iter(range(2, len(node.inputs)))
         g, u = [next(at) if there else None for there in self.given]
-        return rc or lib.thx_token_logprob_train_call(_at(ins, 0), _at(ins, 1), _at(ins, g), _at(ins, u), self.temperature,
-                                                      _at(outs, 0), _at(outs, 1), _at(outs, 2), _at(outs, 3),
-                                                      ws.ptr if ws else None, size, flags)
+        return lib.thx_token_logprob_train_call, (
+            _at(ins, 0), _at(ins, 1), _at(ins, g), _at(ins, u), self.temperature, _at(outs, 0), _at(outs, 1), _at(outs, 2),
+            _at(outs, 3)), (lib.thx_token_logprob_workspace, _at(ins, 0), 0)
 
 
 class HipTopKDistillationTrain(_TrainOp, Op):
@@ -184,11 +230,10 @@ class HipTopKDistillationTrain(_TrainOp, Op):
         self.temperature = float(temperature)
         self.forward = HipTopKDistillation(temperature)
 
-    def call(self, node, ins, outs, flags):
-        rc, ws, size = self.workspace(node, ins, lib.thx_topk_distill_workspace)
-        return rc or lib.thx_topk_distill_train_call(_at(ins, 0), _at(ins, 1), _at(ins, 2), _at(ins, 3), self.temperature,
-                                                     _at(outs, 0), _at(outs, 1), _at(outs, 2), ws.ptr if ws else None,
-                                                     size, flags)
+    def call(self, node, ins, outs):
+        return lib.thx_topk_distill_train_call, (
+            _at(ins, 0), _at(ins, 1), _at(ins, 2), _at(ins, 3), self.temperature, _at(outs, 0), _at(outs, 1),
+            _at(outs, 2)), (lib.thx_topk_distill_workspace, _at(ins, 0))
 
 
 class _Apart(object):

@@ -178,8 +178,14 @@ def sync():
 def stream():
     """The library's one stream as an integer (``hipStream_t``): what a program that uses streams of its own - or
     another library's, ``torch.cuda.ExternalStream(stream())`` - orders its work against."""
-    init()
-    return lib.thx_stream()
+    global _stream
+    if _stream is None:
+        init()
+        _stream = lib.thx_stream()
+    return _stream
+
+
+_stream = None
 
 
 def last_plan():
@@ -449,10 +455,11 @@ class HipArray(object):
     def __cuda_array_interface__(self):
         """The view other libraries take of this array without a copy (``torch.as_tensor(a, device="cuda")``).  They
         have to order their work after the work in ``stream()``, which the entry ``stream`` names."""
-        if self.dtype.kind == "V" or self.buffer.fake:
+        if self.buffer.fake:
             raise AttributeError("__cuda_array_interface__")
-        return {"shape": self.shape, "typestr": self.dtype.str, "data": (self.ptr if self.size else 0, False),
-                "strides": None if self.c_contiguous else self.strides, "version": 3, "stream": lib.thx_stream()}
+        return {"shape": self.shape, "typestr": self.dtype.str,
+                "data": (0 if 0 in self.shape else self.buffer.ptr + self.offset, False), "strides": self.strides,
+                "version": 3, "stream": stream()}
 
     # -- properties
     @property
