@@ -19,9 +19,7 @@ template <int TPR> struct Block { enum { threads = TPR > 256 ? TPR : 256, rows =
 template <int TPR, int N, class A>
 THX_DEV void row_sums(A (&v)[N], A* lds, int& turn) {
 #pragma unroll
-  for (int m = (TPR < 64 ? TPR : 64) / 2; m >= 1; m >>= 1)
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], m, 64);
+  for (int k = 0; k < N; ++k) v[k] = lanes_sum<(TPR < 64 ? TPR : 64)>(v[k]);
   if constexpr (TPR > 64) {
     constexpr int W = TPR / 64;
     A* set = lds + (turn * Block<TPR>::rows + threadIdx.x / TPR) * N * W;
@@ -300,8 +298,7 @@ __global__ void __launch_bounds__(1024) ln_join(const A* partial, int blocks, in
 
 template <class A>
 THX_DEV A block_sum(A v, A* lds) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  v = lanes_sum<64>(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x / 64] = v;
   __syncthreads();

@@ -128,11 +128,10 @@ struct LaneSums {
     if (ENT) w += o.w;
   }
   THX_DEV void join_lanes(A c) {
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-      const A om = __shfl_xor(m, k, 64), os = __shfl_xor(s, k, 64), ow = ENT ? (A)__shfl_xor(w, k, 64) : (A)0;
-      join(om, os, ow, c);
-    }
+    const A all = wave_largest(m);
+    if (all > m) raise(all, c);
+    s = lanes_sum<64>(s);
+    if (ENT) w = lanes_sum<64>(w);
   }
   // A row of nothing but -infinity (a NaN makes the sum a NaN).
   THX_DEV bool nothing_left() const { return m == neg_inf<A>() && s == (A)0; }
@@ -228,11 +227,15 @@ struct Best {
       rank[i] = 0;
     }
     const int used = (n + 63) / 64;
-    for (int j = 0; j < n; ++j) {
-      const Key other = list[j];
+    for (int j = 0; j < n; j += 4) {  // four entries on their way at once
+      Key other[4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) other[a] = list[j + a < n ? j + a : n - 1];
 #pragma unroll
       for (int i = 0; i < kList / 64; ++i)
-        if (i < used) rank[i] += other > key[i];
+        if (i < used)
+#pragma unroll
+          for (int a = 0; a < 4; ++a) rank[i] += j + a < n && other[a] > key[i];
     }
     wave_fence();
 #pragma unroll
@@ -318,7 +321,7 @@ THX_DEV void read_part(const T* x, int64_t cols, int64_t lo, int64_t hi, typenam
     }
   }
   if constexpr (TOP) {
-    best.tighten(sum.m);
+    if (steps * 2 != next) best.tighten(sum.m);  // not right behind the last time
     best.sweep();
     best.sort(best.k);
   }
@@ -438,8 +441,7 @@ THX_DEV void finish(const KdRow<T>& q, const T* x, int64_t cols, int64_t r, type
     const int64_t id = load_index(t.ids, t.i64, r * t.is + k);
     if (id >= 0) loss += entry_loss(q, load_real<A>(t.logits, t.dtype, r * t.ls + k), id, x, cols, c, sum, ls, ts.m, tls);
   }
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) loss += __shfl_xor(loss, k, 64);
+  loss = lanes_sum<64>(loss);
   if (sum.s != sum.s) loss = sum.s;
   if (lane == 0) {
     q.loss[r] = loss * q.t2;
@@ -501,22 +503,10 @@ __global__ void __launch_bounds__(64 * kWaves) vocab_read(Cut<T> q, Row row) {
   }
 }
 
-// The largest key of the wave.
-template <class Key>
-THX_DEV Key wave_max(Key v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    Key o;
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(Key) / 4); ++i) ((unsigned*)&o)[i] = (unsigned)__shfl_xor((int)((unsigned*)&v)[i], m, 64);
-    v = o > v ? o : v;
-  }
-  return v;
-}
-
 // One wave per row over its parts (at most 64: one to a lane).
 template <class T, bool TOP, class Row, bool ENT>
 __global__ void __launch_bounds__(64) vocab_join(Cut<T> q, Row row) {
+  typedef typename AccOf<T>::type A;
   typedef typename Order<T>::Key Key;
   __shared__ Key lists[TOP ? kList : 1];
   const int lane = threadIdx.x;
@@ -534,19 +524,33 @@ __global__ void __launch_bounds__(64) vocab_join(Cut<T> q, Row row) {
       if constexpr (TOP) {
         const int k = row.n_top;
         best.init(lists, k);
+        // Each lane goes down the falling list of its part.  Where there are at least k parts, k entries are no less than
+        // the k-th largest first entry; where the list fills up all the same, its k best are kept.
         const Key* mine = q.lists + (r * q.parts + lane) * k;
-        int at = 0;
-        Key head = lane < q.parts ? mine[0] : (Key)0;
-        for (int i = 0; i < k; ++i) {
-          const Key top = wave_max(head);
-          if (top == (Key)0) break;
-          if (lane == 0) best.list[i] = top;
-          best.n = i + 1;
-          if (head == top) {
-            ++at;
-            head = at < k ? mine[at] : (Key)0;
+        Key at_hand[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) at_hand[i] = lane < q.parts && i < k ? mine[i] : (Key)0;
+        const Key head = at_hand[0];
+        best.tighten(head ? Order<T>::inverse(Order<T>::value_of(head)) : neg_inf<A>());
+        const typename Order<T>::Value least = Order<T>::value(best.reached);
+        Key beyond = 0;
+        for (int i = 0; i < k; i += 4) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const Key key = at_hand[j];
+            at_hand[j] = lane < q.parts && i + 4 + j < k ? mine[i + 4 + j] : (Key)0;
+            const bool take = key > beyond && Order<T>::value_of(key) >= least;
+            if (__ballot(take) && best.n + 64 > kList) {
+              wave_fence();
+              best.sort(k);
+              beyond = best.list[k - 1];
+            }
+            best.append(take && key > beyond, key);
           }
+          if (!__ballot(at_hand[0] > beyond && Order<T>::value_of(at_hand[0]) >= least)) break;
         }
+        wave_fence();
+        best.sort(k);
         wave_fence();
       }
       finish<T, TOP>(row, x, q.cols, r, q.c, sum, best);
@@ -865,8 +869,7 @@ vocab_train(GradCut<T> q, Row row) {
         val[k] = -gt * acc_exp2((e - ts.m) * q.c - tls);
         if (j >= 0) loss += entry_loss(o, e, j, x, q.cols, q.c, sum, ls, ts.m, tls);
       }
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) loss += __shfl_xor(loss, k, 64);
+      loss = lanes_sum<64>(loss);
       if (lane == 0) losses[wave] = loss;
       if (threadIdx.x == 0) {
         o.stats[4 * r] = sum.m;

@@ -63,18 +63,17 @@ class _State(object):
         for v, slot in zip(inputs, self.in_slots):
             v.as_thx(slot)
         shapes = [tuple(s) for s in self.op.infer_shape(self.node, [v.shape for v in inputs])]
-        self.results, at, together = [], 0, []
-        for k, (shape, dtype) in enumerate(zip(shapes, self.dtypes)):
+        self.results, at = [], 0
+        for shape, dtype in zip(shapes, self.dtypes):
             nbytes = dtype.itemsize
             for s in shape:
                 nbytes *= s
             if nbytes <= self._SHARED:
-                together.append(k)
                 offset, at = at, at + (nbytes + 63) // 64 * 64
             else:
                 offset = None
             self.results.append((shape, _c_strides(shape, dtype.itemsize), dtype, _CODE_OF[dtype], nbytes, offset))
-        self.shared_bytes = at
+        self.shared_bytes = max(at, 1) if any(r[5] is not None for r in self.results) else 0
         for (shape, strides, dtype, code, nbytes, offset), slot in zip(self.results, self.out_slots):
             slot.offset_bytes, slot.nd, slot.dtype = offset or 0, len(shape), code
             slot.shape[:len(shape)] = shape
