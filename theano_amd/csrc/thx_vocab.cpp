@@ -292,9 +292,12 @@ THX_DEV void read_part(const T* x, int64_t cols, int64_t lo, int64_t hi, typenam
     for (int u = 1; u < kUnroll; ++u) m = m > vm[u] ? m : vm[u];
     if (m > sum.m) sum.raise(m, c);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < kUnroll; ++u) {
 #pragma unroll
       for (int e = 0; e < V; ++e) sum.add((A)v[u].v[e], c);
+      // one vector after the other: with 32 exponentials at once the half-precision kernel takes 181 registers, not 116
+      if constexpr (TOP && sizeof(T) < 8) asm volatile("" : "+v"(sum.s), "+v"(sum.w));
+    }
     if constexpr (TOP) {
       if (++steps == next) {
         best.tighten(sum.m);
@@ -400,28 +403,39 @@ struct KdRow {
   A *loss, *stats;
 };
 
-// Entry k of the teacher into its sums: nothing where it stands for no token, NaN where it names one that is not there,
-// which makes the row's loss and gradient NaN.
+// An entry of the teacher: its token (-1 for none) and logit.
+template <class A> struct Entry { int64_t id; A logit; };
 template <class A>
-THX_DEV void take_entry(const Teacher<A>& t, int64_t r, int k, int64_t cols, A c, LaneSums<A, false>& ts) {
-  const int64_t id = load_index(t.ids, t.i64, r * t.is + k);
-  if (id < 0) return;
-  const A v = load_real<A>(t.logits, t.dtype, r * t.ls + k);
-  if (v > ts.m) ts.raise(v, c);
-  ts.add(v, c);
-  if (id >= cols) ts.s = (A)NAN;
+THX_DEV Entry<A> load_entry(const Teacher<A>& t, int64_t r, int k) {
+  return {load_index(t.ids, t.i64, r * t.is + k), load_real<A>(t.logits, t.dtype, r * t.ls + k)};
 }
 
-// q (log q - log p) of an entry with logit v and token id >= 0; 0 where q is.
+// An entry into the teacher's sums: nothing where it stands for no token, NaN where it names one that is not there, which
+// makes the row's loss and gradient NaN.
+template <class A>
+THX_DEV void take_entry(const Entry<A>& e, int64_t cols, A c, LaneSums<A, false>& ts) {
+  if (e.id < 0) return;
+  if (e.logit > ts.m) ts.raise(e.logit, c);
+  ts.add(e.logit, c);
+  if (e.id >= cols) ts.s = (A)NAN;
+}
+
+// q (log q - log p) of an entry, `at` being its column's logit; 0 where q is, or where it stands for no token.
 template <class T, class A>
-THX_DEV A entry_loss(const KdRow<T>& q, A v, int64_t id, const T* x, int64_t cols, A c, const LaneSums<T, false>& sum, A ls,
-                     A tm, A tls) {
-  if (tm == neg_inf<A>() && tls == neg_inf<A>()) return 0;
-  const A p = acc_exp2((v - tm) * c - tls);
+THX_DEV A entry_loss(const KdRow<T>& q, const Entry<A>& e, T at, int64_t cols, A c, const LaneSums<T, false>& sum, A ls, A tm,
+                     A tls) {
+  if (e.id < 0 || (tm == neg_inf<A>() && tls == neg_inf<A>())) return 0;
+  const A p = acc_exp2((e.logit - tm) * c - tls);
   if (p == (A)0) return 0;
-  if (id >= cols) return (A)NAN;
-  const A lp = sum.nothing_left() ? neg_inf<A>() : log_prob(x[id], sum.m, c, q.inv_t, ls);
-  return p * (log_prob(v, tm, c, q.inv_t, tls) - lp);
+  if (e.id >= cols) return (A)NAN;
+  const A lp = sum.nothing_left() ? neg_inf<A>() : log_prob(at, sum.m, c, q.inv_t, ls);
+  return p * (log_prob(e.logit, tm, c, q.inv_t, tls) - lp);
+}
+
+// The logit of an entry's column, anything where it has none.
+template <class T, class A>
+THX_DEV T entry_at(const Entry<A>& e, const T* x, int64_t cols) {
+  return e.id >= 0 && e.id < cols ? x[e.id] : (T)0;
 }
 
 template <class T>
@@ -433,13 +447,13 @@ THX_DEV void finish(const KdRow<T>& q, const T* x, int64_t cols, int64_t r, type
   const A ls = sum.log2_sum();
   LaneSums<A, false> ts;  // the teacher's side: entries as single or double precision
   ts.init();
-  for (int k = lane; k < t.n; k += 64) take_entry(t, r, k, cols, c, ts);
+  for (int k = lane; k < t.n; k += 64) take_entry(load_entry(t, r, k), cols, c, ts);
   ts.join_lanes(c);
   const A tls = ts.log2_sum();
   A loss = 0;
   for (int k = lane; k < t.n; k += 64) {
-    const int64_t id = load_index(t.ids, t.i64, r * t.is + k);
-    if (id >= 0) loss += entry_loss(q, load_real<A>(t.logits, t.dtype, r * t.ls + k), id, x, cols, c, sum, ls, ts.m, tls);
+    const Entry<A> e = load_entry(t, r, k);
+    loss += entry_loss(q, e, entry_at(e, x, cols), cols, c, sum, ls, ts.m, tls);
   }
   loss = lanes_sum<64>(loss);
   if (sum.s != sum.s) loss = sum.s;
@@ -683,21 +697,35 @@ struct RowSlope {
   }
 };
 
-// The elements of columns [first, last) that the list names, written over; behind a barrier.
+// Element j of a row's gradient, which entry k of the list names, written over; behind a barrier.  The first entry of a
+// column writes for all that name it.
+template <class T, class A>
+THX_DEV void write_entry(const RowSlope<T>& slope, T at, T* dx, const int* id, const A* val, int n, int k, int j) {
+  A v = 0;
+  int before = 0, i = 0;
+  for (; i + 4 <= n; i += 4) {  // four at a time: each is a wait for LDS
+    const int4 o = *(const int4*)(id + i);
+    if (o.x == j || o.y == j || o.z == j || o.w == j) {
+      v += (o.x == j ? val[i] : (A)0) + (o.y == j ? val[i + 1] : (A)0) + (o.z == j ? val[i + 2] : (A)0) +
+           (o.w == j ? val[i + 3] : (A)0);
+      before |= (i < k && o.x == j) | (i + 1 < k && o.y == j) | (i + 2 < k && o.z == j) | (i + 3 < k && o.w == j);
+    }
+  }
+  for (; i < n; ++i)
+    if (id[i] == j) {
+      v += val[i];
+      before |= i < k;
+    }
+  if (!before) dx[j] = (T)(slope(at) + v);
+}
+
+// All elements of columns [first, last) that the list names.
 template <class T, class A>
 THX_DEV void write_entries(const RowSlope<T>& slope, const T* x, T* dx, const int* id, const A* val, int n, int64_t first,
-                           int64_t last) {
-  for (int k = threadIdx.x; k < n; k += blockDim.x) {
+                           int64_t last, int from = 0) {
+  for (int k = from + threadIdx.x; k < n; k += blockDim.x) {
     const int j = id[k];
-    if (j < first || j >= last) continue;
-    A v = 0;
-    bool mine = true;
-    for (int i = 0; i < n; ++i)
-      if (id[i] == j) {
-        v += val[i];
-        if (i < k) mine = false;
-      }
-    if (mine) dx[j] = (T)(slope(x[j]) + v);
+    if (j >= first && j < last) write_entry(slope, x[j], dx, id, val, n, k, j);
   }
 }
 
@@ -705,7 +733,7 @@ template <class T, class Row>
 __global__ void __launch_bounds__(256) vocab_grad(GradCut<T> q, Row row) {
   typedef typename AccOf<T>::type A;
   constexpr int V = Width<T>::value;
-  __shared__ int id[Row::kEntries];
+  __shared__ __align__(16) int id[Row::kEntries];
   __shared__ A val[Row::kEntries];
   const int64_t units = q.rows * q.segs, whole = q.cols / V, vectors = (q.cols + V - 1) / V;
   for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
@@ -768,7 +796,7 @@ vocab_train(GradCut<T> q, Row row) {
   constexpr int V = Width<T>::value, W = THREADS / 64;
   constexpr bool ENT = Row::kEntropy;
   constexpr int G = VPT % 4 ? (VPT % 2 ? 1 : 2) : 4;  // vectors between two looks at the maximum
-  __shared__ int id[Row::kEntries];
+  __shared__ __align__(16) int id[Row::kEntries];
   __shared__ A val[Row::kEntries];
   __shared__ A part[W][ENT ? 3 : 4], losses[W];
   const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
@@ -778,6 +806,16 @@ vocab_train(GradCut<T> q, Row row) {
     const T* x = q.x + r * q.xs;
     T* dx = q.dx + r * q.cols;
     const T* xt = x + (int)threadIdx.x * V;
+    // a teacher's entry to each thread, on its way before the row: what hangs on it is not waited for behind the row
+    [[maybe_unused]] int mine_id = -1;  // the row's length where it names a column that is not there
+    [[maybe_unused]] A mine_logit = neg_inf<A>();
+    [[maybe_unused]] T mine_at = (T)0;
+    if constexpr (!ENT) {
+      if ((int)threadIdx.x < row.out.t.n) {
+        const Entry<A> e = load_entry(row.out.t, r, threadIdx.x);
+        mine_id = (int)(e.id < 0 ? -1 : e.id < q.cols ? e.id : q.cols), mine_logit = e.logit;
+      }
+    }
     Vec<T, V> v[VPT];
 #pragma unroll
     for (int u = 0; u < VPT; ++u) {
@@ -792,6 +830,7 @@ vocab_train(GradCut<T> q, Row row) {
     // the elements behind the last whole vector, one to a thread
     const bool extra = (int)threadIdx.x < rest;
     const T tail = extra ? x[(int64_t)whole * V + threadIdx.x] : (T)neg_inf<A>();
+    if constexpr (!ENT) mine_at = entry_at<T, A>({mine_id, mine_logit}, x, q.cols);
     LaneSums<T, ENT> sum;
     sum.init();
     if ((A)tail > sum.m) sum.raise((A)tail, q.c);
@@ -821,7 +860,9 @@ vocab_train(GradCut<T> q, Row row) {
     [[maybe_unused]] LaneSums<A, false> ts;
     if constexpr (!ENT) {
       ts.init();
-      for (int k = threadIdx.x; k < row.out.t.n; k += THREADS) take_entry(row.out.t, r, k, q.cols, q.c, ts);
+      take_entry({mine_id, mine_logit}, q.cols, q.c, ts);
+      for (int k = threadIdx.x + THREADS; k < row.out.t.n; k += THREADS)
+        take_entry(load_entry(row.out.t, r, k), q.cols, q.c, ts);
       ts.join_lanes(q.c);
       if (lane == 0) part[wave][2] = ts.m, part[wave][3] = ts.s;
     }
@@ -862,12 +903,15 @@ vocab_train(GradCut<T> q, Row row) {
       const A tls = ts.log2_sum(), gt = row.g[r * row.gs] * row.temperature;
       s.a = tls != tls ? tls : ts.nothing_left() ? (A)0 : gt;
       A loss = 0;
-      for (int k = threadIdx.x; k < n; k += THREADS) {
-        const int64_t j = load_index(t.ids, t.i64, r * t.is + k);
-        const A e = load_real<A>(t.logits, t.dtype, r * t.ls + k);
-        id[k] = j >= 0 && j < q.cols && !ts.nothing_left() ? (int)j : -1;
-        val[k] = -gt * acc_exp2((e - ts.m) * q.c - tls);
-        if (j >= 0) loss += entry_loss(o, e, j, x, q.cols, q.c, sum, ls, ts.m, tls);
+      auto put = [&](int k, const Entry<A>& e, T at) {
+        id[k] = e.id >= 0 && e.id < q.cols && !ts.nothing_left() ? (int)e.id : -1;
+        val[k] = -gt * acc_exp2((e.logit - ts.m) * q.c - tls);
+        loss += entry_loss(o, e, at, q.cols, q.c, sum, ls, ts.m, tls);
+      };
+      if ((int)threadIdx.x < n) put(threadIdx.x, {mine_id, mine_logit}, mine_at);
+      for (int k = threadIdx.x + THREADS; k < n; k += THREADS) {
+        const Entry<A> e = load_entry(t, r, k);
+        put(k, e, entry_at(e, x, q.cols));
       }
       loss = lanes_sum<64>(loss);
       if (lane == 0) losses[wave] = loss;
@@ -889,8 +933,14 @@ vocab_train(GradCut<T> q, Row row) {
     }
     if (extra) dx[(int64_t)whole * V + threadIdx.x] = slope.none ? (T)0 : (T)slope(tail);
     __syncthreads();  // the entries and the losses are there, and the elements that the entries replace are written
-    if (!slope.none) write_entries(slope, x, dx, id, val, n, 0, q.cols);
-    if constexpr (!ENT) {
+    if constexpr (ENT) {
+      if (!slope.none) write_entries(slope, x, dx, id, val, n, 0, q.cols);
+    } else {
+      if (!slope.none) {
+        const int j = (int)threadIdx.x < n ? id[threadIdx.x] : -1;
+        if (j >= 0) write_entry(slope, mine_at, dx, id, val, n, threadIdx.x, j);
+        write_entries(slope, x, dx, id, val, n, 0, q.cols, THREADS);
+      }
       if (threadIdx.x == 0) {
         A loss = losses[0];
         for (int w = 1; w < W; ++w) loss += losses[w];
