@@ -790,8 +790,7 @@ struct KdTrain {
 };
 
 template <class T, class Row, int THREADS, int VPT>
-__global__ void __launch_bounds__(THREADS, THREADS == 1024 && VPT <= 8 && sizeof(T) < 8 ? 8 : 1)
-vocab_train(GradCut<T> q, Row row) {
+__global__ void __launch_bounds__(THREADS, VPT > 8 && sizeof(T) < 8 ? 4 : 1) vocab_train(GradCut<T> q, Row row) {
   typedef typename AccOf<T>::type A;
   constexpr int V = Width<T>::value, W = THREADS / 64;
   constexpr bool ENT = Row::kEntropy;
@@ -877,6 +876,7 @@ vocab_train(GradCut<T> q, Row row) {
     const A ls = sum.log2_sum();
     Slope<A> s = {sum.m, ls, (A)0, (A)0};
     int n;
+    [[maybe_unused]] A tls, gt;
     if constexpr (ENT) {
       const LpRow<T>& o = row.out;
       n = 1;
@@ -898,23 +898,9 @@ vocab_train(GradCut<T> q, Row row) {
       }
     } else {
       const KdRow<T>& o = row.out;
-      const Teacher<A>& t = o.t;
-      n = t.n;
-      const A tls = ts.log2_sum(), gt = row.g[r * row.gs] * row.temperature;
+      n = o.t.n;
+      tls = ts.log2_sum(), gt = row.g[r * row.gs] * row.temperature;
       s.a = tls != tls ? tls : ts.nothing_left() ? (A)0 : gt;
-      A loss = 0;
-      auto put = [&](int k, const Entry<A>& e, T at) {
-        id[k] = e.id >= 0 && e.id < q.cols && !ts.nothing_left() ? (int)e.id : -1;
-        val[k] = -gt * acc_exp2((e.logit - ts.m) * q.c - tls);
-        loss += entry_loss(o, e, at, q.cols, q.c, sum, ls, ts.m, tls);
-      };
-      if ((int)threadIdx.x < n) put(threadIdx.x, {mine_id, mine_logit}, mine_at);
-      for (int k = threadIdx.x + THREADS; k < n; k += THREADS) {
-        const Entry<A> e = load_entry(t, r, k);
-        put(k, e, entry_at(e, x, q.cols));
-      }
-      loss = lanes_sum<64>(loss);
-      if (lane == 0) losses[wave] = loss;
       if (threadIdx.x == 0) {
         o.stats[4 * r] = sum.m;
         o.stats[4 * r + 1] = ls;
@@ -932,6 +918,22 @@ vocab_train(GradCut<T> q, Row row) {
       if (u < full || u * THREADS + (int)threadIdx.x < whole) store_out(dt + u * (THREADS * V), o[0], q.nt);
     }
     if (extra) dx[(int64_t)whole * V + threadIdx.x] = slope.none ? (T)0 : (T)slope(tail);
+    if constexpr (!ENT) {  // behind the stores: the registers that held the row are free
+      const KdRow<T>& o = row.out;
+      A loss = 0;
+      auto put = [&](int k, const Entry<A>& e, T at) {
+        id[k] = e.id >= 0 && e.id < q.cols && !ts.nothing_left() ? (int)e.id : -1;
+        val[k] = -gt * acc_exp2((e.logit - ts.m) * q.c - tls);
+        loss += entry_loss(o, e, at, q.cols, q.c, sum, ls, ts.m, tls);
+      };
+      if ((int)threadIdx.x < n) put(threadIdx.x, {mine_id, mine_logit}, mine_at);
+      for (int k = threadIdx.x + THREADS; k < n; k += THREADS) {
+        const Entry<A> e = load_entry(o.t, r, k);
+        put(k, e, entry_at(e, x, q.cols));
+      }
+      loss = lanes_sum<64>(loss);
+      if (lane == 0) losses[wave] = loss;
+    }
     __syncthreads();  // the entries and the losses are there, and the elements that the entries replace are written
     if constexpr (ENT) {
       if (!slope.none) write_entries(slope, x, dx, id, val, n, 0, q.cols);
@@ -1023,16 +1025,21 @@ int launch_grad(const Rows& x, double temperature, const Rows& dx, Row row, cons
   return launch_builtin((const void*)&vocab_grad<T, Row>, plan, dim3(grid_of(x.rows * q.segs)), dim3(256), args);
 }
 
-// The block that holds a row of the one-pass kernel: threads, and vectors to a thread; 0 where none does.
+// The block that holds a row of the one-pass kernel: threads, and vectors to a thread; 0 where none does.  Two blocks of a
+// compute unit hide each other's waits, so 512 threads with up to 20 vectors (no more than 128 registers) come before 1024:
+// 4877 rows of 50257 halves in 512x16 211 us, in 1024x8 215 (228 and 254 with 64 teacher's entries, where 64 registers do
+// not do); 3000 rows of 80000 in 512x20 200 us, in 1024x16 240.  Up to 4096 vectors 8 to a thread leave room for four
+// blocks: 8192 rows of 32000 halves in 512x8 192 us, in 256x16 210.  Doubles take a third more registers, and no more than
+// 8192 vectors.
 struct Hold {
   int threads = 0, vpt = 0;
 };
 Hold hold_of(const Rows& x) {
-  static const Hold all[] = {{256, 1}, {256, 2}, {256, 4}, {256, 8}, {512, 8}, {1024, 8}, {1024, 16}, {1024, 20}};
+  static const Hold all[] = {{256, 1}, {256, 2}, {256, 4}, {256, 8}, {512, 8}, {512, 16}, {512, 20}, {1024, 16}, {1024, 20}};
   const int isz = dtype_size(x.dtype);
   const int64_t whole = x.cols / (16 / isz);  // the elements behind the last whole vector go to one thread each
   for (const Hold& h : all)
-    if (whole <= (int64_t)h.threads * h.vpt && !(isz == 8 && h.vpt > 8)) return h;
+    if (whole <= (int64_t)h.threads * h.vpt && !(isz == 8 && h.vpt * h.threads > 8192)) return h;
   return Hold();
 }
 
@@ -1057,10 +1064,12 @@ int launch_train(const Rows& x, double temperature, const Rows& dx, const Hold& 
     case 256 * 32 + 4: kernel = (const void*)&vocab_train<T, Row, 256, 4>; break;
     case 256 * 32 + 8: kernel = (const void*)&vocab_train<T, Row, 256, 8>; break;
     case 512 * 32 + 8: kernel = (const void*)&vocab_train<T, Row, 512, 8>; break;
-    case 1024 * 32 + 8: kernel = (const void*)&vocab_train<T, Row, 1024, 8>; break;
+    case 512 * 32 + 16: kernel = (const void*)&vocab_train<T, Row, 512, 16>; break;
     default:
       if constexpr (sizeof(T) < 8)
-        kernel = h.vpt == 16 ? (const void*)&vocab_train<T, Row, 1024, 16> : (const void*)&vocab_train<T, Row, 1024, 20>;
+        kernel = h.threads == 512  ? (const void*)&vocab_train<T, Row, 512, 20>
+                 : h.vpt == 16 ? (const void*)&vocab_train<T, Row, 1024, 16>
+                               : (const void*)&vocab_train<T, Row, 1024, 20>;
   }
   return launch_builtin(kernel, plan, dim3(grid_of(x.rows)), dim3(h.threads), args);
 }
