@@ -571,6 +571,37 @@ def test_topk_distillation(shape, k, dtype, tdt, idt):
     check_kd(x, teacher, ids, g=g, what="some masked")
 
 
+@pytest.mark.parametrize("vectors", [256, 512, 1024, 2048, 4096, 8192, 10240, 16384, 20480])
+@pytest.mark.parametrize("dtype", ["float16", "float32", "float64"])
+def test_rows_as_long_as_a_block_holds(dtype, vectors):
+    """A loss with its gradient in one launch keeps a row in a block's registers: the last row that a block of each size
+    holds, and the first that it does not."""
+    rng = np.random.default_rng(vectors)
+    width = 16 // np.dtype(dtype).itemsize
+    for cols in (vectors * width, vectors * width + width):
+        x = logits(rng, (2, cols), dtype)
+        tokens = np.array([cols - 1, 0])
+        w, u = [rng.standard_normal(2).astype(acc_of(dtype)) for _ in range(2)]
+        check_lp(x, tokens, w=w, u=u, what=str(cols))
+        ids = rng.integers(0, cols, (2, 70))
+        ids[:, :4] = cols - 1, 0, cols - 1, cols - 2
+        ids[0, 69] = 0
+        check_kd(x, rng.standard_normal((2, 70)).astype("float32"), ids, g=w, temperature=1.5, what=str(cols))
+
+
+@pytest.mark.parametrize("entries", [3, 4, 5, 255, 256, 257, 1024])
+def test_entries_that_name_the_same_columns(entries):
+    """Many entries to a column, at both ends of the list and of a block's turns through it."""
+    rng = np.random.default_rng(entries)
+    for dtype, cols in (("float16", 40), ("float32", 2100), ("float16", 33000)):
+        ids = rng.integers(0, 6, (3, entries)).astype("int32")      # six columns share the entries
+        ids[1] = cols - 1
+        ids[2, 1:-1] = -1
+        ids[2, -1] = ids[2, 0]
+        check_kd(logits(rng, (3, cols), dtype), rng.standard_normal((3, entries)).astype("float16"), ids,
+                 g=rng.standard_normal(3).astype("float32"), what="%s %d" % (dtype, cols))
+
+
 # ---- gradients against differences, and the operators together ---------------------------------------------
 
 def differences(f, args, k, h):
