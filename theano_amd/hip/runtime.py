@@ -348,6 +348,7 @@ def _c_strides(shape, itemsize):
 
 
 _CODE_OF = dict((np.dtype(name), scal.dtype_code(name)) for name in scal.all_dtypes)
+_OF_TYPESTR = dict((d.str, (d, code)) for d, code in _CODE_OF.items())   # native byte order alone
 
 
 class HipArray(object):
@@ -441,15 +442,16 @@ class HipArray(object):
         d = obj.__cuda_array_interface__
         if d.get("mask") is not None:
             raise TypeError("a masked array cannot be viewed as a HipArray")
-        dtype, shape, strides = np.dtype(d["typestr"]), tuple(d["shape"]), d.get("strides")
-        if dtype not in _CODE_OF or not dtype.isnative:
-            raise TypeError("dtype %s is not supported on the device" % dtype)
+        dtype, code = _OF_TYPESTR.get(d["typestr"], (None, None))
+        if dtype is None:
+            raise TypeError("dtype %s is not supported on the device" % np.dtype(d["typestr"]))
+        shape, strides = tuple(d["shape"]), d.get("strides")
         if len(shape) > THX_MAX_ND:
             raise TypeError("arrays of rank %d exceed the limit of %d" % (len(shape), THX_MAX_ND))
         if 0 in shape:
             return cls.empty(shape, dtype)
         strides = _c_strides(shape, dtype.itemsize) if strides is None else tuple(strides)
-        return cls._raw(_Foreign(obj, d["data"][0]), 0, shape, strides, dtype, _CODE_OF[dtype])
+        return cls._raw(_Foreign(obj, d["data"][0]), 0, shape, strides, dtype, code)
 
     @property
     def __cuda_array_interface__(self):
