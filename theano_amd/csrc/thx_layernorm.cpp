@@ -58,6 +58,25 @@ THX_DEV void store_edge(T* p, const Vec<T, V>& v, int64_t i, int64_t cols, bool 
   }
 }
 
+// A thread's V sums of columns, `left` of which are there.
+template <class P, class A, int V>
+THX_DEV void store_sums(P* p, const A (&v)[V], int64_t left) {
+  constexpr int W = Width<P>::value < V ? Width<P>::value : V;
+  if (left >= V) {
+#pragma unroll
+    for (int e = 0; e < V; e += W) {
+      Vec<P, W> o;
+#pragma unroll
+      for (int k = 0; k < W; ++k) o.v[k] = (P)v[e + k];
+      store_out(p + e, o, false);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < left) p[e] = (P)v[e];
+  }
+}
+
 THX_DEV float rsqrt_of(float v) { return 1.0f / sqrtf(v); }
 THX_DEV double rsqrt_of(double v) { return 1.0 / sqrt(v); }
 
@@ -154,7 +173,8 @@ __global__ void __launch_bounds__(Block<TPR>::threads) ln_backward(const T* x, i
                                                                    int64_t rows, int64_t cols, const P* gamma,
                                                                    const typename AccOf<T>::type* mean, int64_t ms,
                                                                    const typename AccOf<T>::type* invstd, int64_t is, T* dx,
-                                                                   typename AccOf<T>::type* partial, bool nt) {
+                                                                   typename AccOf<T>::type* partial, P* dgamma, P* dbeta,
+                                                                   bool nt) {
   typedef typename AccOf<T>::type A;
   constexpr int V = Width<T>::value, RPB = Block<TPR>::rows;
   __shared__ A lds[TPR > 64 ? 4 * Block<TPR>::threads / 64 : 1];
@@ -248,14 +268,15 @@ __global__ void __launch_bounds__(Block<TPR>::threads) ln_backward(const T* x, i
         }
       }
       if (group == 0) {
-        A* to = partial + (int64_t)blockIdx.x * 2 * cols;
         const int64_t j = (int64_t)(u * TPR + t) * V;
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (j + e < cols) {
-            to[j + e] = dg[u][e];
-            to[cols + j + e] = db[u][e];
-          }
+        if (gridDim.x == 1) {  // nothing to join
+          store_sums(dgamma + j, dg[u], cols - j);
+          if (dbeta) store_sums(dbeta + j, db[u], cols - j);
+        } else {
+          A* to = partial + (int64_t)blockIdx.x * 2 * cols + j;
+          store_sums(to, dg[u], cols - j);
+          store_sums(to + cols, db[u], cols - j);
+        }
       }
     }
   }
@@ -439,7 +460,10 @@ int64_t forward_blocks(const Shape& s, int64_t rows) {
 
 // Every block leaves one set of sums for ln_join, so no more of them than it takes to keep the memory busy: rows of 4096
 // halves, 256 x 2, with 1, 2 and 4 blocks to a compute unit 133, 89 and 108 us; rows of 512, 64 x 1, 185, 113 and 84.
+// What one block does in four turns it does alone, and writes the gradients itself: 4 rows of 4096 halves 9.2 us, where
+// four blocks take 6.1 and ln_join 6.2; 8 rows in one block 14 us.
 int64_t backward_blocks(const Shape& s, int64_t rows) {
+  if (rows <= 4 * (s.tpr > 256 ? 1 : 256 / s.tpr)) return 1;
   return even_blocks(s, rows, (int64_t)compute_units() * (s.tpr > 256 ? 1 : s.vpt > 1 ? 2 : 4));
 }
 
@@ -617,7 +641,8 @@ int layernorm_grad(const thx_array* x, const thx_array* dy, const thx_array* gam
       rc = by_back_shape(shape, [&](auto h) {
         constexpr int TPR = decltype(h)::tpr, VPT = decltype(h)::vpt;
         void* args[] = {&in[0].ptr, &in[0].stride, &in[1].ptr, &in[1].stride, &in[0].rows, &in[0].cols, &in[4].ptr,
-                        &in[2].ptr, &in[2].stride, &in[3].ptr, &in[3].stride, &out[0].ptr, &ws, &nt};
+                        &in[2].ptr, &in[2].stride, &in[3].ptr, &in[3].stride, &out[0].ptr, &ws, &out[1].ptr, &out[2].ptr,
+                        &nt};
         const void* kernel = dgamma ? (const void*)&ln_backward<T, P, TPR, VPT, true>
                                     : (const void*)&ln_backward<T, P, TPR, VPT, false>;
         return launch_builtin(kernel, plan, dim3(blocks), dim3(Block<TPR>::threads), args);
@@ -635,7 +660,7 @@ int layernorm_grad(const thx_array* x, const thx_array* dy, const thx_array* gam
                             args);
       }
     }
-    if (rc || !dgamma) return rc;
+    if (rc || !dgamma || (shape.tpr && blocks == 1)) return rc;
     void* join[] = {&ws, &blocks, &in[0].cols, &out[1].ptr, &out[2].ptr};
     return launch_builtin((const void*)&ln_join<A, P>, plan + "|join", dim3(columns, dbeta ? 2 : 1), dim3(1024), join);
   });
