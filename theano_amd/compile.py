@@ -226,6 +226,7 @@ class Function(object):
 
     def _prepare(self):
         from .hip.opt import DeviceConstant
+        from .hip.ops import HostToHip
         from .hip.runtime import HipArray
         # storage cells
         self.storage = {}
@@ -282,12 +283,13 @@ class Function(object):
             self.thunks.append((_guarded(node.op.perform) if self.nan_guard else node.op.perform, node,
                                 [self.storage[i] for i in node.inputs],
                                 [self.storage[o] for o in node.outputs], node in static,
-                                self.release[len(self.thunks)]))
+                                self.release[len(self.thunks)], type(node.op) is HostToHip and not self.nan_guard))
         self._static_key = None
         self._input_cells = [self.storage[v] for v in self.fgraph.inputs]
         self._constants_ready = False
         self._HipArray = HipArray
         self._last_shape = {}
+        self._last_device_shape = {}
 
     def _shape_only_nodes(self):
         """Host nodes whose results depend on nothing but the shapes of the function's arguments: the
@@ -350,6 +352,9 @@ class Function(object):
                 continue
             if isinstance(a, HipArray) and isinstance(var.type, TensorType):
                 # device-resident argument for a host-typed input: checked like a host value
+                if a.shape == self._last_device_shape.get(var) and a.dtype == var.type.numpy_dtype:
+                    self.storage[var][0] = a
+                    continue
                 if a.dtype != var.type.numpy_dtype or len(a.shape) != var.type.ndim:
                     raise TypeError("Bad input argument %s: expected %s, got %s" % (spec.name, var.type, a))
                 for d, b in enumerate(var.type.broadcastable):
@@ -357,6 +362,7 @@ class Function(object):
                         raise TypeError("Non-unit value on shape on a broadcastable dimension.", a.shape,
                                         var.type.broadcastable)
                 self.storage[var][0] = a
+                self._last_device_shape[var] = a.shape
             else:
                 try:
                     v = self.storage[var][0] = var.type.filter(a, strict=spec.strict, allow_downcast=spec.allow_downcast)
@@ -383,10 +389,13 @@ class Function(object):
         key = tuple([getattr(c[0], "shape", None) for c in self._input_cells])
         same = key == self._static_key and None not in key
         self._static_key = None                 # stays unset if a node raises half-way
-        for perform, node, ins, outs, static, release in self.thunks:
+        for perform, node, ins, outs, static, release, upload in self.thunks:
             if static and same:
                 continue
-            perform(node, [c[0] for c in ins], outs)
+            if upload and type(ins[0][0]) is HipArray:
+                outs[0][0] = ins[0][0]      # on the device already
+            else:
+                perform(node, [c[0] for c in ins], outs)
             for cell in release:
                 cell[0] = None
         self._static_key = key
