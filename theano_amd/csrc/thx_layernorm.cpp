@@ -459,7 +459,7 @@ int64_t forward_blocks(const Shape& s, int64_t rows) {
 }
 
 // Every block leaves one set of sums for ln_join, so no more of them than it takes to keep the memory busy: rows of 4096
-// halves, 256 x 2, with 1, 2 and 4 blocks to a compute unit 133, 89 and 108 us; rows of 512, 64 x 1, 185, 113 and 84.
+// halves, 256 x 2, with 2, 3 and 4 blocks to a compute unit 82, 85 and 89 us, and ln_join 8 to 11.
 // What one block does in four turns it does alone, and writes the gradients itself: 4 rows of 4096 halves 9.2 us, where
 // four blocks take 6.1 and ln_join 6.2; 8 rows in one block 14 us.
 int64_t backward_blocks(const Shape& s, int64_t rows) {
