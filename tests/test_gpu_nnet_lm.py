@@ -781,6 +781,62 @@ def test_the_same_call_gives_the_same_bits():
                 np.testing.assert_array_equal(a, b.to_numpy())
 
 
+def test_offsets_past_32_bits():
+    """More than 2^31 elements, and rows further apart than 2^31: the rows at both ends and on both sides of the border,
+    the others holding whatever the memory held."""
+    rng = np.random.default_rng(29)
+
+    def rows_of(a, ids):
+        return np.stack([HipArray(a.buffer, a.offset + r * a.strides[0], a.shape[1:], a.strides[1:], a.dtype).to_numpy()
+                         for r in ids])
+
+    def put(a, ids, values):
+        for r, v in zip(ids, values):
+            copy_into(HipArray.from_numpy(v), HipArray(a.buffer, a.offset + r * a.strides[0], a.shape[1:], a.strides[1:], a.dtype))
+
+    def compare(got, ref, ids, names, n):
+        for g, name in zip(got, names):
+            v = rows_of(g, ids)
+            if name == "top_at":
+                np.testing.assert_array_equal(v, ref[name])
+            elif name in ref:
+                close(v, *ref[name], n, name, "float32")
+
+    big = HipArray.empty(((1 << 31) + 40 * 131073,), "float16")
+    for V in (131073, 999):
+        rows = big.size // V if V > 1000 else 3
+        step = V if V > 1000 else (big.size - V) // 2 // 8 * 8 - 5      # 999: three rows a thousand million apart
+        x = HipArray(big.buffer, 0, (rows, V), (2 * step, 2), "float16")
+        ids = sorted(set([0, 1, (1 << 31) // step - 1, (1 << 31) // step, rows - 2, rows - 1]) & set(range(rows)))
+        v = logits(rng, (len(ids), V), "float16")
+        put(x, ids, v)
+        tokens = rng.integers(0, V, rows)
+        w, u = [rng.standard_normal(rows).astype("float32") for _ in range(2)]
+        ref = lp_ref(v, tokens[ids], w=w[ids], u=u[ids])
+        for fuse in (True, False):
+            got = lp_function("float16", "int64", 2, 0, 1.0, (True, True, False), fuse)(x, tokens, w, u)
+            compare(got, ref, ids, ["log_prob", "entropy", "dx"], chain(V))
+            del got
+        got = lp_function("float16", "int64", 2, 5, 1.0, (False,) * 3)(x, tokens)
+        compare(got, lp_ref(v, tokens[ids], n_top=5), ids, ["log_prob", "entropy", "top", "top_at"], chain(V))
+        teacher, at = rng.standard_normal((rows, 3)).astype("float32"), rng.integers(0, V, (rows, 3))
+        ref = kd_ref(v, teacher[ids], at[ids], g=w[ids])
+        for fuse in (True, False):
+            got = kd_function("float16", "float32", "int64", 2, 1.0, True, fuse)(x, teacher, at, w)
+            compare(got, ref, ids, ["loss", "dx"], chain(V) + 3)
+            del got
+    for V in (4097, 70000):          # rows in registers, and the kernels for any row
+        rows = big.size // V
+        x = HipArray(big.buffer, 0, (rows, V), (2 * V, 2), "float16")
+        ids = [0, 1, (1 << 31) // V - 1, (1 << 31) // V, rows - 1]
+        v = rng.standard_normal((len(ids), V)).astype("float16")
+        put(x, ids, v)
+        gamma, beta = [rng.standard_normal(V).astype("float32") for _ in range(2)]
+        got = ln_function("float16", "float32", 2, 2, 1e-5, True)(x, gamma, beta, x)
+        compare(got, ln_ref(v, gamma, beta, 1e-5, v), ids, ["y", "mean", "invstd", "dx"], chain(V))
+        del got
+
+
 # ---- arrays of other libraries -----------------------------------------------------------------------------
 
 def test_views_of_and_for_other_libraries():
