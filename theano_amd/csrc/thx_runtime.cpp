@@ -528,10 +528,10 @@ int launch_builtin(const void* kernel, const std::string& plan, dim3 grid, dim3 
   THX_HIP_CHECK(hipGetDevice(&current));
   if (current != r.device) THX_HIP_CHECK(hipSetDevice(r.device));
   ProfRec rec;
-  rec.plan = plan;
   hipError_t e = hipSuccess;
   if (g_profiling) {
-    if (e == hipSuccess) e = hipEventCreate(&rec.a);
+    rec.plan = plan;
+    e = hipEventCreate(&rec.a);
     if (e == hipSuccess) e = hipEventCreate(&rec.b);
     if (e == hipSuccess) e = hipEventRecord(rec.a, r.stream);
   }

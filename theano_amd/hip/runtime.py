@@ -7,6 +7,7 @@ plays for the reference (``theano/gpuarray/type.py:129-517``): a strided view
 (shape, byte strides, offset) over a reference-counted device buffer.
 """
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -299,6 +300,10 @@ class capture(object):
         return False
 
 
+# what every call uses, looked up once
+_alloc, _free, _void_p, _byref = lib.thx_alloc, lib.thx_free, ctypes.c_void_p, ctypes.byref
+
+
 class _Buffer(object):
     """One pooled device allocation, released when the last view dies."""
 
@@ -311,9 +316,12 @@ class _Buffer(object):
             self.ptr = _fake_next[0]
             _fake_next[0] += (self.nbytes + 4095) // 4096 * 4096 + 4096
             return
-        init()
-        p = ctypes.c_void_p()
-        check(lib.thx_alloc(max(int(nbytes), 1), ctypes.byref(p)))
+        if not _initialised:
+            init()
+        p = _void_p()
+        rc = _alloc(self.nbytes or 1, _byref(p))
+        if rc:
+            check(rc)
         self.ptr = p.value
         if _capture_keep is not None:
             _capture_keep.append(self)
@@ -321,7 +329,7 @@ class _Buffer(object):
     def __del__(self):
         try:
             if self.ptr and not self.fake:
-                lib.thx_free(self.ptr)
+                _free(self.ptr)
                 self.ptr = None
         except Exception:
             pass
@@ -349,6 +357,8 @@ def _c_strides(shape, itemsize):
 
 _CODE_OF = dict((np.dtype(name), scal.dtype_code(name)) for name in scal.all_dtypes)
 _OF_TYPESTR = dict((d.str, (d, code)) for d, code in _CODE_OF.items())   # native byte order alone
+_TYPESTR_OF = dict((code, d.str) for d, code in _CODE_OF.items())
+_c_strides_of = functools.lru_cache(1024)(_c_strides)   # of shapes that come again with every call
 
 
 class HipArray(object):
@@ -450,18 +460,20 @@ class HipArray(object):
             raise TypeError("arrays of rank %d exceed the limit of %d" % (len(shape), THX_MAX_ND))
         if 0 in shape:
             return cls.empty(shape, dtype)
-        strides = _c_strides(shape, dtype.itemsize) if strides is None else tuple(strides)
+        strides = _c_strides_of(shape, dtype.itemsize) if strides is None else tuple(strides)
         return cls._raw(_Foreign(obj, d["data"][0]), 0, shape, strides, dtype, code)
 
     @property
     def __cuda_array_interface__(self):
         """The view other libraries take of this array without a copy (``torch.as_tensor(a, device="cuda")``).  They
-        have to order their work after the work in ``stream()``, which the entry ``stream`` names."""
-        if self.buffer.fake:
+        have to order their work after the work in ``stream()``, which the entry ``stream`` names, and to have finished
+        it, or ordered it before that stream's further work, when they let the array go: its memory is used again."""
+        buffer, shape = self.buffer, self.shape
+        if buffer.fake:
             raise AttributeError("__cuda_array_interface__")
-        return {"shape": self.shape, "typestr": self.dtype.str,
-                "data": (0 if 0 in self.shape else self.buffer.ptr + self.offset, False), "strides": self.strides,
-                "version": 3, "stream": stream()}
+        return {"shape": shape, "typestr": _TYPESTR_OF[self.code],
+                "data": (0 if 0 in shape else buffer.ptr + self.offset, False), "strides": self.strides,
+                "version": 3, "stream": _stream or stream()}
 
     # -- properties
     @property
