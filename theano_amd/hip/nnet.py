@@ -54,7 +54,11 @@ class _State(object):
         self.outs = (thx_array * len(node.outputs))()
         self.in_slots, self.out_slots = list(self.ins), list(self.outs)
         self.dtypes = [np.dtype(o.type.dtype) for o in node.outputs]
-        self.fn, self.args, self.query = op.call(node, self.ins, self.outs)
+        fn, args, self.query = op.call(node, self.ins, self.outs)
+        # the call without the declared types, whose check of every argument costs more than the library's: all that is
+        # passed is made here or below, as what the declaration says (an int is a C int)
+        self.fn = lib[fn.__name__]
+        self.args = tuple(ctypes.c_double(a) if isinstance(a, float) else a for a in args)
         self.layout = None
 
     def plan(self, inputs, layout):
@@ -79,13 +83,11 @@ class _State(object):
             slot.shape[:len(shape)] = shape
             slot.strides_bytes[:len(shape)] = strides
         mark_reused(self.node, self.ins, self.outs)
-        self.workspace = 0
+        self.workspace = ctypes.c_size_t()
         if self.query is not None:
-            n = ctypes.c_size_t()
-            rc = self.query[0](*(self.query[1:] + (ctypes.byref(n),)))
+            rc = self.query[0](*(self.query[1:] + (ctypes.byref(self.workspace),)))
             if rc:
                 return rc
-            self.workspace = n.value
         self.layout = layout
         return 0
 
@@ -109,8 +111,8 @@ class _State(object):
                 rc = self.fn(*self.args, flags)
             else:
                 # kept for the length of the call alone, or by the recording the call is made in
-                ws = _Buffer(self.workspace) if self.workspace else None
-                rc = self.fn(*self.args, ws.ptr if ws else None, self.workspace, flags)
+                ws = _Buffer(self.workspace.value) if self.workspace.value else None
+                rc = self.fn(*self.args, ctypes.c_void_p(ws.ptr) if ws else None, self.workspace, flags)
             if not rc:
                 return results
         if rc == _UNSUPPORTED:          # rows at more than one stride, or columns apart
