@@ -276,6 +276,13 @@ int thx_layernorm_grad_call(const thx_array* x, const thx_array* dy, const thx_a
                             const thx_array* invstd, const thx_array* dx, const thx_array* dgamma,
                             const thx_array* dbeta, void* workspace, size_t workspace_bytes, int flags);
 
+/* thx_layernorm_call and thx_layernorm_grad_call in one, for a dy that is known beforehand: x and dy are read once.  The
+ * workspace is that of the gradient call. */
+int thx_layernorm_train_call(const thx_array* x, const thx_array* dy, const thx_array* gamma, const thx_array* beta,
+                             double epsilon, const thx_array* y, const thx_array* mean, const thx_array* invstd,
+                             const thx_array* dx, const thx_array* dgamma, const thx_array* dbeta, void* workspace,
+                             size_t workspace_bytes, int flags);
+
 #define THX_MAX_TOP 64        /* alternatives per row of thx_token_logprob_call */
 #define THX_MAX_TEACHER 1024  /* entries per row of thx_topk_distill_call */
 

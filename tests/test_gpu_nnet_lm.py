@@ -174,8 +174,9 @@ def tensor(dtype, nd, name=None):
 _cache = {}
 
 
-def ln_function(dtype, pdtype, nd, n_params, eps, train):
-    key = ("ln", dtype, pdtype, nd, n_params, eps, train)
+def ln_function(dtype, pdtype, nd, n_params, eps, train, fuse=True):
+    """``fuse``: the forward pass and the gradients in one launch, else two."""
+    key = ("ln", dtype, pdtype, nd, n_params, eps, train, fuse)
     if key not in _cache:
         x, dy = tensor(dtype, nd), tensor(dtype, nd)
         ps = [tensor(pdtype, 1) for _ in range(n_params)]
@@ -184,7 +185,7 @@ def ln_function(dtype, pdtype, nd, n_params, eps, train):
         if train:
             outs += th.grad(None, ins, known_grads={outs[0]: dy})
             ins = ins + [dy]
-        _cache[key] = th.function(ins, [Out(o, device=True) for o in outs])
+        _cache[key] = th.function(ins, [Out(o, device=True) for o in outs], fuse=fuse)
     return _cache[key]
 
 
@@ -217,13 +218,19 @@ def kd_function(dtype, tdt, idt, nd, temperature, train, fuse=True):
 
 def check_ln(x, gamma, beta, dy=None, eps=1e-5, dev=None, what=""):
     """``dev``: device arrays that hold the same values in another layout, by position of the argument."""
+    ref = ln_ref(x, gamma, beta, eps, dy)
+    for fuse in ([True, False] if dy is not None else [False]):
+        check_ln_call(x, gamma, beta, dy, eps, dev, ref, fuse, what)
+
+
+def check_ln_call(x, gamma, beta, dy, eps, dev, ref, fuse, what):
     ps = [p for p in (gamma, beta) if p is not None]
-    f = ln_function(str(x.dtype), str(ps[0].dtype) if ps else "float32", x.ndim, len(ps), eps, dy is not None)
+    f = ln_function(str(x.dtype), str(ps[0].dtype) if ps else "float32", x.ndim, len(ps), eps, dy is not None, fuse)
+    assert any(type(n.op).__name__ == "HipLayerNormalizationTrain" for n in f.toposort()) == fuse
     args = [x] + ps + ([dy] if dy is not None else [])
     for k, v in (dev or {}).items():
         args[k] = v
     got = [o.to_numpy() for o in f(*args)]
-    ref = ln_ref(x, gamma, beta, eps, dy)
     names = ["y", "mean", "invstd"] + (["dx", "dgamma", "dbeta"][:1 + len(ps)] if dy is not None else [])
     acc = acc_of(str(x.dtype))
     assert len(got) == len(names)
@@ -832,9 +839,11 @@ def test_offsets_past_32_bits():
         v = rng.standard_normal((len(ids), V)).astype("float16")
         put(x, ids, v)
         gamma, beta = [rng.standard_normal(V).astype("float32") for _ in range(2)]
-        got = ln_function("float16", "float32", 2, 2, 1e-5, True)(x, gamma, beta, x)
-        compare(got, ln_ref(v, gamma, beta, 1e-5, v), ids, ["y", "mean", "invstd", "dx"], chain(V))
-        del got
+        ref = ln_ref(v, gamma, beta, 1e-5, v)
+        for fuse in (True, False):
+            got = ln_function("float16", "float32", 2, 2, 1e-5, True, fuse)(x, gamma, beta, x)
+            compare(got, ref, ids, ["y", "mean", "invstd", "dx"], chain(V))
+            del got
 
 
 # ---- arrays of other libraries -----------------------------------------------------------------------------

@@ -92,6 +92,29 @@ def test_what_the_vocabulary_operators_refuse():
         nnet.topk_distillation_loss(x, x, x)
 
 
+def test_layer_normalization_with_a_known_gradient_is_one_node(dry_run):
+    x, g, b, dy = T.fmatrix(), T.fvector(), T.fvector(), T.fmatrix()
+    y, mean, invstd = nnet.layer_normalization(x, g, b)
+    norms = lambda f: [n for n in device_nodes(f) if n.startswith("HipLayer")]       # noqa: E731
+    one, two = ["HipLayerNormalizationTrain"], ["HipLayerNormalization", "HipLayerNormalizationGrad"]
+    known = th.grad(None, [x, g, b], known_grads={y: dy})
+    assert norms(th.function([x, g, b, dy], [y, mean] + known)) == one
+    assert norms(th.function([x, g, b, dy], known)) == one
+    assert norms(th.function([x, g, b, dy], known, fuse=False)) == two
+    assert norms(th.function([x, g, b], th.grad(T.sum(y), [x, g, b]))) == one
+    # a gradient that hangs on the result, or on the statistics
+    assert norms(th.function([x, g, b], th.grad(T.sum(T.sqr(y)), x))) == two
+    assert norms(th.function([x, g, b, dy], th.grad(None, x, known_grads={y: dy * mean.dimshuffle(0, "x")}))) == two
+    # of two layers the second alone
+    z = nnet.layer_normalization(y, g)[0]
+    f = th.function([x, g, b, dy], th.grad(None, [x, g, b], known_grads={z: dy}))
+    assert sorted(norms(f)) == sorted(one + two)
+    # statistics of another call on the same rows are not its own
+    other = nnet.layer_normalization(x, g, b, epsilon=1e-3)
+    f = th.function([x, g, b, dy], known + [other[0]])
+    assert sorted(norms(f)) == sorted(one + two[:1])
+
+
 def test_narrow_token_types_are_converted():
     for dt in ("int8", "uint8", "int16", "uint16", "uint32", "uint64"):
         assert nnet.token_log_probs(T.fmatrix(), tensor(dt, 1))[0].type.dtype == "float32"
@@ -101,7 +124,7 @@ def test_gradient_graphs(dry_run):
     """One node per pass: results that nothing uses cost nothing, and their missing gradients are not made up."""
     x, g, b = T.fmatrix(), T.fvector(), T.fvector()
     y = nnet.layer_normalization(x, g, b)[0]
-    f = th.function([x, g, b], th.grad(T.sum(y), [x, g, b]))
+    f = th.function([x, g, b], th.grad(T.sum(y), [x, g, b]), fuse=False)
     names = device_nodes(f)
     assert names.count("HipLayerNormalization") == 1 and names.count("HipLayerNormalizationGrad") == 1
     t, w = T.lvector(), T.fvector()

@@ -165,6 +165,46 @@ __global__ void __launch_bounds__(Block<TPR>::threads) ln_forward(const T* x, in
   }
 }
 
+// A block's sums of the parameters' gradients: the gradients themselves where it is the only one.
+template <int TPR, int VPT, class P, class A, int V>
+THX_DEV void leave_sums(A (&dg)[VPT][V], A (&db)[VPT][V], int group, int t, int64_t cols, A* partial, P* dgamma, P* dbeta) {
+  constexpr int RPB = Block<TPR>::rows;
+  // the groups of a block first, through LDS, one column vector at a time
+  constexpr int VEC = V * 2;
+  __shared__ A fold[RPB > 1 ? RPB * TPR * VEC : 1];
+#pragma unroll
+  for (int u = 0; u < VPT; ++u) {
+    if constexpr (RPB > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        fold[(2 * e) * RPB * TPR + threadIdx.x] = dg[u][e];
+        fold[(2 * e + 1) * RPB * TPR + threadIdx.x] = db[u][e];
+      }
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          for (int k = 1; k < RPB; ++k) {
+            dg[u][e] += fold[(2 * e) * RPB * TPR + k * TPR + t];
+            db[u][e] += fold[(2 * e + 1) * RPB * TPR + k * TPR + t];
+          }
+      }
+    }
+    if (group == 0) {
+      const int64_t j = (int64_t)(u * TPR + t) * V;
+      if (gridDim.x == 1) {  // nothing to join
+        store_sums(dgamma + j, dg[u], cols - j);
+        if (dbeta) store_sums(dbeta + j, db[u], cols - j);
+      } else {
+        A* to = partial + (int64_t)blockIdx.x * 2 * cols + j;
+        store_sums(to, dg[u], cols - j);
+        store_sums(to + cols, db[u], cols - j);
+      }
+    }
+  }
+}
+
 // The gradients.  A block goes through rows blockIdx.x, + gridDim.x, ... (RPB of them at a time) and keeps the sums of
 // dy * xhat and dy of its rows in registers, per column; at the end it leaves them in partial[block][2][cols], which
 // ln_join adds up.  One pass over x and dy serves all three gradients.
@@ -244,42 +284,97 @@ __global__ void __launch_bounds__(Block<TPR>::threads) ln_backward(const T* x, i
       store_edge(out, o, i, cols, nt);
     }
   }
-  if constexpr (PARAMS) {
-    // the groups of a block first, through LDS, one column vector at a time
-    constexpr int VEC = V * 2;
-    __shared__ A fold[RPB > 1 ? RPB * TPR * VEC : 1];
+  if constexpr (PARAMS) leave_sums<TPR, VPT>(dg, db, group, t, cols, partial, dgamma, dbeta);
+}
+
+// Forward and all gradients in one, for a dy that is known beforehand: a row and its dy are read once.  The sums behind
+// dx need no invstd until they are there, sum(a xhat) = invstd sum(a (x - mean)), so that the row's sums come together in
+// two steps: the mean, then the squares around it beside both others.
+template <class T, class P, int TPR, int VPT, bool PARAMS>
+__global__ void __launch_bounds__(Block<TPR>::threads) ln_train(const T* x, int64_t xs, const T* dy, int64_t ds, int64_t rows,
+                                                                int64_t cols, const P* gamma, const P* beta, double eps, T* y,
+                                                                typename AccOf<T>::type* mean,
+                                                                typename AccOf<T>::type* invstd, T* dx,
+                                                                typename AccOf<T>::type* partial, P* dgamma, P* dbeta, bool nt) {
+  typedef typename AccOf<T>::type A;
+  constexpr int V = Width<T>::value, RPB = Block<TPR>::rows, WAVES = Block<TPR>::threads / 64;
+  __shared__ A lds_mean[TPR > 64 ? 2 * WAVES : 1], lds[TPR > 64 ? 6 * WAVES : 1];
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  const A share = (A)1 / (A)cols;
+  int turn_mean = 0, turn = 0;
+  A dg[VPT][V], db[VPT][V];
+#pragma unroll
+  for (int u = 0; u < VPT; ++u)
+#pragma unroll
+    for (int e = 0; e < V; ++e) dg[u][e] = db[u][e] = 0;
+  constexpr bool AHEAD = TPR < 1024 || V * VPT < 16;
+  auto row_at = [&](int64_t r0) { return r0 + group < rows ? r0 + group : rows - 1; };
+  Vec<T, V> v[VPT], d[VPT], vn[VPT], dn[VPT];
+  Vec<P, V> g[VPT];
+  auto load = [&](int64_t r) {
 #pragma unroll
     for (int u = 0; u < VPT; ++u) {
-      if constexpr (RPB > 1) {
-        __syncthreads();
+      load_edge(vn[u], x + r * xs, u * TPR + t, cols);
+      load_edge(dn[u], dy + r * ds, u * TPR + t, cols);
+    }
+  };
+  if (AHEAD && (int64_t)blockIdx.x * RPB < rows) load(row_at((int64_t)blockIdx.x * RPB));
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          fold[(2 * e) * RPB * TPR + threadIdx.x] = dg[u][e];
-          fold[(2 * e + 1) * RPB * TPR + threadIdx.x] = db[u][e];
-        }
-        __syncthreads();
-        if (group == 0) {
+  for (int u = 0; u < VPT; ++u)
+    if (gamma) load_edge(g[u], gamma, u * TPR + t, cols);
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    const bool live = r0 + group < rows;
+    const int64_t r = row_at(r0);
+    if (!AHEAD) load(r);
 #pragma unroll
-          for (int e = 0; e < V; ++e)
-            for (int k = 1; k < RPB; ++k) {
-              dg[u][e] += fold[(2 * e) * RPB * TPR + k * TPR + t];
-              db[u][e] += fold[(2 * e + 1) * RPB * TPR + k * TPR + t];
-            }
-        }
-      }
-      if (group == 0) {
-        const int64_t j = (int64_t)(u * TPR + t) * V;
-        if (gridDim.x == 1) {  // nothing to join
-          store_sums(dgamma + j, dg[u], cols - j);
-          if (dbeta) store_sums(dbeta + j, db[u], cols - j);
-        } else {
-          A* to = partial + (int64_t)blockIdx.x * 2 * cols + j;
-          store_sums(to, dg[u], cols - j);
-          store_sums(to + cols, db[u], cols - j);
-        }
+    for (int u = 0; u < VPT; ++u) v[u] = vn[u], d[u] = dn[u];
+    if (AHEAD && r0 + (int64_t)gridDim.x * RPB < rows) load(row_at(r0 + (int64_t)gridDim.x * RPB));
+    A sum[1] = {0};
+#pragma unroll
+    for (int u = 0; u < VPT; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[0] += (A)v[u].v[e];
+    row_sums<TPR>(sum, lds_mean, turn_mean);
+    const A mu = sum[0] * share;
+    A s[3] = {0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      const int64_t left = cols - (int64_t)(u * TPR + t) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const A dv = (A)d[u].v[e], a = gamma ? dv * (A)g[u].v[e] : dv, xc = (A)v[u].v[e] - mu;
+        s[0] += e < left ? xc * xc : (A)0;
+        s[1] += a;
+        s[2] += a * xc;
       }
     }
+    row_sums<TPR>(s, lds, turn);
+    const A inv = rsqrt_of(s[0] * share + (A)eps), s0 = s[1] * share, s1 = s[2] * share * inv;
+    T *yr = y + r * cols, *out = dx + r * cols;
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+      const int64_t i = u * TPR + t;
+      if (i * V >= cols) continue;
+      Vec<P, V> b;
+      if (beta) load_edge(b, beta, i, cols);
+      Vec<T, V> o, z;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const A dv = (A)d[u].v[e], gv = gamma ? (A)g[u].v[e] : (A)1, xh = ((A)v[u].v[e] - mu) * inv;
+        const A w = gamma ? xh * gv : xh;
+        z.v[e] = (T)(beta ? w + (A)b.v[e] : w);
+        o.v[e] = (T)(inv * ((gamma ? dv * gv : dv) - s0 - xh * s1));
+        if (PARAMS && live) {
+          dg[u][e] += dv * xh;
+          db[u][e] += dv;
+        }
+      }
+      store_edge(yr, z, i, cols, nt);
+      store_edge(out, o, i, cols, nt);
+    }
+    if (t == 0) mean[r] = mu, invstd[r] = inv;
   }
+  if constexpr (PARAMS) leave_sums<TPR, VPT>(dg, db, group, t, cols, partial, dgamma, dbeta);
 }
 
 // Adds up the blocks' sums: 64 columns by 16 slices of the blocks to a block here, blockIdx.y 0 for gamma, 1 for beta.
@@ -666,6 +761,61 @@ int layernorm_grad(const thx_array* x, const thx_array* dy, const thx_array* gam
   });
 }
 
+int layernorm_train(const thx_array* x, const thx_array* dy, const thx_array* gamma, const thx_array* beta, double epsilon,
+                    const thx_array* y, const thx_array* mean, const thx_array* invstd, const thx_array* dx,
+                    const thx_array* dgamma, const thx_array* dbeta, void* ws, size_t ws_bytes, int flags) {
+  const char* what = "layer normalization with gradients";
+  const bool dry = (flags & THX_DRY_RUN) != 0;
+  // what the two calls look at, then what lies between them
+  int rc = layernorm(x, gamma, beta, epsilon, y, mean, invstd, flags | THX_DRY_RUN);
+  if (rc) return rc;
+  if ((rc = layernorm_grad(x, dy, gamma, mean, invstd, dx, dgamma, dbeta, ws, ws_bytes, flags | THX_DRY_RUN))) return rc;
+  Rows in[4], out[6];
+  const thx_array* ins[4] = {x, dy, gamma, beta};
+  const thx_array* outs[6] = {y, mean, invstd, dx, dgamma, dbeta};
+  for (int k = 0; k < 4; ++k)
+    if (ins[k] && (rc = rows_of(what, "an operand", ins[k], -1, k < 2, flags, &in[k]))) return rc;
+  for (int k = 0; k < 6; ++k)
+    if (outs[k] && (rc = rows_of(what, "a result", outs[k], -1, k == 0 || k == 3, flags, &out[k]))) return rc;
+  if ((rc = no_overlap(what, out, 6, in, 4)) && !dry) return rc;
+  size_t need = 0;
+  if ((rc = layernorm_grad_bytes(x, dgamma, &need))) return rc;
+  if ((rc = check_workspace(what, ws, ws_bytes, need, flags))) return rc;
+  const int64_t cols = in[0].cols;
+  const bool packed = cols <= 1 || ((!gamma || in[2].stride == 1) && (!beta || in[3].stride == 1));
+  const Shape shape = shape_of(cols, in[0].dtype, true, packed);
+  // Two launches for rows that no block holds, and where a block of 1024 has no registers left for both passes and many
+  // rows to go through: 2048 rows of 16384 halves 83 us, in one launch 92 (of 8192 halves 70 and 64, of 8192 floats 130
+  // and 113, 16384 rows of 4096 halves 137 and 126).
+  const bool crowded = in[0].dtype == THX_F16 && shape.tpr == 1024 && shape.vpt == 2 && dgamma && in[0].rows > compute_units();
+  if (!shape.tpr || crowded) {
+    if ((rc = layernorm(x, gamma, beta, epsilon, y, mean, invstd, flags))) return rc;
+    return layernorm_grad(x, dy, gamma, mean, invstd, dx, dgamma, dbeta, ws, ws_bytes, flags);
+  }
+  const std::string plan = plan_of("lnt", in[0].dtype, shape);
+  set_last_plan(plan);
+  if (dry) return THX_OK;
+  if ((rc = ensure_init())) return rc;
+  bool nt = stream_out(in[0], out[3]);
+  return by_types(in[0].dtype, gamma ? in[2].dtype : in[0].dtype, [&](auto t, auto p) {
+    typedef decltype(t) T;
+    typedef decltype(p) P;
+    typedef typename AccOf<T>::type A;
+    int blocks = (int)backward_blocks(shape, in[0].rows);
+    int rc = by_back_shape(shape, [&](auto h) {
+      constexpr int TPR = decltype(h)::tpr, VPT = decltype(h)::vpt;
+      void* args[] = {&in[0].ptr, &in[0].stride, &in[1].ptr, &in[1].stride, &in[0].rows, &in[0].cols, &in[2].ptr, &in[3].ptr,
+                      &epsilon, &out[0].ptr, &out[1].ptr, &out[2].ptr, &out[3].ptr, &ws, &out[4].ptr, &out[5].ptr, &nt};
+      const void* kernel = dgamma ? (const void*)&ln_train<T, P, TPR, VPT, true> : (const void*)&ln_train<T, P, TPR, VPT, false>;
+      return launch_builtin(kernel, plan, dim3(blocks), dim3(Block<TPR>::threads), args);
+    });
+    if (rc || !dgamma || blocks == 1) return rc;
+    void* join[] = {&ws, &blocks, &in[0].cols, &out[4].ptr, &out[5].ptr};
+    return launch_builtin((const void*)&ln_join<A, P>, plan + "|join", dim3(grid_of((cols + 63) / 64), dbeta ? 2 : 1), dim3(1024),
+                          join);
+  });
+}
+
 }  // namespace
 }  // namespace thx
 
@@ -687,6 +837,15 @@ int thx_layernorm_grad_call(const thx_array* x, const thx_array* dy, const thx_a
                             const thx_array* dbeta, void* workspace, size_t workspace_bytes, int flags) {
   return guarded("thx_layernorm_grad_call", [&] {
     return layernorm_grad(x, dy, gamma, mean, invstd, dx, dgamma, dbeta, workspace, workspace_bytes, flags);
+  });
+}
+
+int thx_layernorm_train_call(const thx_array* x, const thx_array* dy, const thx_array* gamma, const thx_array* beta,
+                             double epsilon, const thx_array* y, const thx_array* mean, const thx_array* invstd,
+                             const thx_array* dx, const thx_array* dgamma, const thx_array* dbeta, void* workspace,
+                             size_t workspace_bytes, int flags) {
+  return guarded("thx_layernorm_train_call", [&] {
+    return layernorm_train(x, dy, gamma, beta, epsilon, y, mean, invstd, dx, dgamma, dbeta, workspace, workspace_bytes, flags);
   });
 }
 

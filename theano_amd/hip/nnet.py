@@ -202,6 +202,35 @@ class _TrainOp(_RowOp):
         return self.forward.infer_shape(node, shapes[:self.n_forward]) + [shapes[0]]
 
 
+class HipLayerNormalizationTrain(_RowOp, Op):
+    """``HipLayerNormalization`` and ``HipLayerNormalizationGrad`` for a ``dy`` that does not depend on the result (the
+    first step back of a part of a model whose forward pass is run again): ``x, dy[, gamma[, beta]]``, then the results
+    of both."""
+
+    __props__ = ("epsilon", "n_params")
+
+    def __init__(self, epsilon, n_params):
+        self.epsilon, self.n_params = float(epsilon), int(n_params)
+
+    def make_node(self, x, dy, *params):
+        x, dy = as_hip_variable(x), as_hip_variable(dy)
+        params = [as_hip_variable(p) for p in params]
+        outs = HipLayerNormalization(self.epsilon).make_node(x, *params).outputs
+        grads = HipLayerNormalizationGrad(self.n_params).make_node(x, dy, outs[1], outs[2], *params[:1]).outputs
+        return Apply(self, [x, dy] + params, [o.type() for o in outs + grads])
+
+    def infer_shape(self, node, shapes):
+        return [shapes[0], shapes[0][:-1], shapes[0][:-1], shapes[0]] + [shapes[2] for _ in range(self.n_params)]
+
+    def call(self, node, ins, outs):
+        n = self.n_params
+        dgamma = _at(outs, 4 if n else None)
+        return lib.thx_layernorm_train_call, (
+            _at(ins, 0), _at(ins, 1), _at(ins, 2 if n else None), _at(ins, 3 if n > 1 else None), self.epsilon, _at(outs, 0),
+            _at(outs, 1), _at(outs, 2), _at(outs, 3), dgamma, _at(outs, 5 if n > 1 else None)), (
+            lib.thx_layernorm_grad_workspace, _at(ins, 0), dgamma)
+
+
 class HipTokenLogProbsTrain(_TrainOp, Op):
     """``HipTokenLogProbs`` without alternatives and ``HipTokenLogProbsGrad``; ``given`` says which of the gradients of
     ``log_prob`` and ``entropy`` follow the logits and the tokens."""
@@ -304,12 +333,35 @@ def _one_value(g):
     return v if isinstance(v.type, HipArrayType) else g
 
 
+def _fuse_layer_normalization(fgraph, node):
+    x, dy, mean, invstd = node.inputs[:4]
+    fwd = mean.owner
+    if fwd is None or not isinstance(fwd.op, HipLayerNormalization) or [mean, invstd] != list(fwd.outputs[1:]):
+        return 0
+    if fwd.inputs[0] is not x or list(fwd.inputs[1:2]) != list(node.inputs[4:5]) or len(fwd.inputs) - 1 != node.op.n_params:
+        return 0
+    dy = _Apart(fwd, lambda: x)(dy)
+    if dy is None:
+        return 0
+    new = HipLayerNormalizationTrain(fwd.op.epsilon, node.op.n_params).make_node(x, dy, *fwd.inputs[1:])
+    old = list(fwd.outputs) + list(node.outputs)
+    if [o.type for o in old] != [o.type for o in new.outputs]:
+        return 0
+    for o, no in reversed(list(zip(old, new.outputs))):
+        fgraph.replace(o, no)
+    return 1
+
+
 def fuse_known_gradients(fgraph):
-    """A forward node over the vocabulary and its gradient node become one where the gradients of the results do not
-    depend on the results: a weighted sum or mean of the losses, not a function such as a ratio of probabilities."""
+    """A forward node and its gradient node become one where the gradients of the results do not depend on the results:
+    a weighted sum or mean of losses, not a function such as a ratio of probabilities; of layer normalisation a gradient
+    that is an argument."""
     count = 0
     for node in fgraph.toposort():
         if node not in fgraph.apply_nodes:
+            continue
+        if isinstance(node.op, HipLayerNormalizationGrad):
+            count += _fuse_layer_normalization(fgraph, node)
             continue
         if isinstance(node.op, HipTokenLogProbsGrad):
             if node.op.given[2]:

@@ -90,6 +90,7 @@ def _load():
         "thx_layernorm_call": ([A, A, A, ctypes.c_double, A, A, A, ctypes.c_int], ctypes.c_int),
         "thx_layernorm_grad_workspace": ([A, A, P(sz)], ctypes.c_int),
         "thx_layernorm_grad_call": ([A] * 8 + [vp, sz, ctypes.c_int], ctypes.c_int),
+        "thx_layernorm_train_call": ([A] * 4 + [ctypes.c_double] + [A] * 6 + [vp, sz, ctypes.c_int], ctypes.c_int),
         "thx_token_logprob_workspace": ([A, ctypes.c_int, P(sz)], ctypes.c_int),
         "thx_token_logprob_call": ([A, A, ctypes.c_double, ctypes.c_int] + [A] * 5 + [vp, sz, ctypes.c_int], ctypes.c_int),
         "thx_token_logprob_grad_call": ([A] * 8 + [ctypes.c_double, A, ctypes.c_int], ctypes.c_int),
