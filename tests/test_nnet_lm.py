@@ -294,6 +294,30 @@ def test_the_library_checks_its_operands():
     refused(lng(g=None), 7, "without gamma")
     refused(lng(dg=None, db=at((8,), "float32")), 7, "without dgamma")
 
+    def lnt(**kw):
+        a = dict(x=at((4, 8), "float32"), dy=at((4, 8), "float32"), g=at((8,), "float32"), b=at((8,), "float32"),
+                 y=at((4, 8), "float32"), m=at((4,), "float32"), i=at((4,), "float32"), dx=at((4, 8), "float32"),
+                 dg=at((8,), "float32"), db=at((8,), "float32"), ws=fake, size=1 << 20, eps=1e-5)
+        a.update((k, a[v] if isinstance(v, str) else v) for k, v in kw.items())
+        r = [None if a[k] is None else ctypes.byref(a[k]) for k in ("x", "dy", "g", "b", "y", "m", "i", "dx", "dg", "db")]
+        return lib.thx_layernorm_train_call(*(r[:4] + [a["eps"]] + r[4:] + [a["ws"], a["size"], 0]))
+
+    refused(lnt(x=None), 7, "missing")
+    refused(lnt(dy=None), 7, "missing")
+    refused(lnt(dy=at((4, 7), "float32")), 2, "mis-match")
+    refused(lnt(dy=at((4, 8), "float16")), 3, "dtype")
+    refused(lnt(dy=arr((4, 8), "float32", base=None)), 7, "no base")
+    refused(lnt(eps=-1.0), 7, "epsilon")
+    refused(lnt(g=None), 7, "without gamma")
+    refused(lnt(dg=None), 7, "without dgamma")
+    refused(lnt(y="dy"), 7, "overlaps")
+    refused(lnt(dx="dy"), 7, "overlaps")
+    refused(lnt(dx="y"), 7, "overlap")
+    refused(lnt(dg="b"), 7, "overlaps")
+    refused(lnt(size=0), 7, "workspace of")
+    refused(lnt(ws=None), 7, "no address")
+    refused(lnt(ws=fake + 8), 7, "16 bytes")
+
     def lp(V=8, t="int64", k=0, temp=1.0, top="yes", rows=4, x=None):
         a = [at((rows, V), "float32") if x is None else x, at((rows,), t)]
         o = [at((rows,), "float32"), at((rows,), "float32"), at((rows, k), "float32") if k > 0 and top else None,
