@@ -667,6 +667,21 @@ def test_one_weight_for_all_rows():
         close(got, a["dx"][0] + b["dx"][0], a["dx"][1] + b["dx"][1] + off / (chain(777) * 2.0 ** -24), chain(777), "dx", "float32")
 
 
+def test_two_results_that_are_each_others_gradients():
+    rng = np.random.default_rng(30)
+    a, b = T.fmatrix(), T.fmatrix()
+    ya, yb = T.nnet.layer_normalization(a)[0], T.nnet.layer_normalization(b)[0]
+    va, vb = [rng.standard_normal((5, 70)).astype("float32") for _ in range(2)]
+    f = th.function([a, b], [th.grad(None, a, known_grads={ya: yb}), th.grad(None, b, known_grads={yb: ya})])
+    got = f(va, vb)
+    la, lb = [ln_ref(v, None, None, 1e-5)["y"][0].astype("float32") for v in (va, vb)]
+    for g, v, dy in zip(got, (va, vb), (lb, la)):
+        # dy is a result itself, off by the same number of roundings of its own scale m (|xhat| + largest |x| * invstd, 2 to
+        # 7 here), where dx counts its value: (m + mean(m) + m mean(m^2)) / (mean|dy| + 2 m mean(|dy| m)) is below 4
+        value, scale = ln_ref(v, None, None, 1e-5, dy)["dx"]
+        close(g, value, scale, 5 * chain(70), "dx", "float32")
+
+
 def test_second_derivatives_of_layer_normalization():
     rng = np.random.default_rng(22)
     x, gamma, beta, z = T.dmatrix(), T.dvector(), T.dvector(), T.dmatrix()

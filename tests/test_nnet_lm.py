@@ -115,6 +115,38 @@ def test_layer_normalization_with_a_known_gradient_is_one_node(dry_run):
     assert sorted(norms(f)) == sorted(one + two[:1])
 
 
+def test_known_gradients_are_looked_for_in_deep_and_shared_graphs(dry_run):
+    """Far more nodes between a result and its gradient than the interpreter nests calls, and far more paths than nodes."""
+    from theano_amd.hip.nnet import _Apart
+    x, g = T.fmatrix(), T.fvector()
+    y = nnet.layer_normalization(x, g)[0]
+    deep, shared = y, y
+    for _ in range(3000):
+        deep = T.tanh(deep)
+    for _ in range(200):
+        shared = shared * shared
+    order = {}
+    for v in (deep, shared):
+        apart = _Apart(y.owner, lambda: x, order)
+        assert apart.depends(v) and not apart.depends(x * 2) and apart(v) is None
+        assert apart(T.second(v, x)) is None                 # the shape of something that far is not looked into
+        assert apart(x * 2).owner.inputs[0] is x
+    z = y
+    for _ in range(60):
+        z = nnet.layer_normalization(z * z + 1, g)[0]
+    f = th.function([x, g], th.grad(T.sum(z), x))
+    assert device_nodes(f).count("HipLayerNormalizationTrain") == 1
+
+
+def test_known_gradients_make_no_cycle(dry_run):
+    """Two results that are each other's gradients: when the one pair has become one node, the other's gradient hangs on it."""
+    a, b = T.fmatrix(), T.fmatrix()
+    ya, yb = nnet.layer_normalization(a)[0], nnet.layer_normalization(b)[0]
+    f = th.function([a, b], [th.grad(None, a, known_grads={ya: yb * 2}), th.grad(None, b, known_grads={yb: ya * 3})])
+    names = [n for n in device_nodes(f) if n.startswith("HipLayer")]
+    assert sorted(names) == ["HipLayerNormalization", "HipLayerNormalizationGrad", "HipLayerNormalizationTrain"]
+
+
 def test_narrow_token_types_are_converted():
     for dt in ("int8", "uint8", "int16", "uint16", "uint32", "uint64"):
         assert nnet.token_log_probs(T.fmatrix(), tensor(dt, 1))[0].type.dtype == "float32"

@@ -270,31 +270,51 @@ class _Apart(object):
     """Rewrites expressions so that they no longer depend on the results of one node, where all they take from them is
     their shape: the fills that sums and means leave in gradients."""
 
-    def __init__(self, node, rows):
+    _DEEP = 64      # such fills are a few nodes; what is deeper stays as it is
+
+    def __init__(self, node, rows, order):
         self.node, self.rows = node, rows     # ``rows``: makes a variable with the shape of the node's results per row
-        self.known, self.model = {}, None
+        self.order = order                    # place of every node of the graph; none ahead of ``node`` depends on it
+        self.free, self.shaped, self.done, self.model = set(), {}, {}, None
 
     def depends(self, v):
-        if v not in self.known:
-            n = v.owner
-            self.known[v] = n is not None and (n is self.node or any(self.depends(i) for i in n.inputs))
-        return self.known[v]
+        """Graphs are deep and their nodes shared: every variable is visited once, without recursion."""
+        place = self.order.get(self.node, -1)
+        seen, todo = set(), [v]
+        while todo:
+            w = todo.pop()
+            n = w.owner
+            if n is self.node:
+                return True
+            if n is None or w in seen or w in self.free or self.order.get(n, place) < place:
+                continue
+            seen.add(w)
+            todo.extend(n.inputs)
+        self.free |= seen
+        return False
 
-    def row_shaped(self, v):
+    def row_shaped(self, v, depth=0):
         """Elementwise over a result of the node, and nowhere broadcast against anything larger."""
-        first = self.node.outputs[0].type
         n = v.owner
-        if n is None or v.type.broadcastable != first.broadcastable:
+        if n is None or depth > self._DEEP or v.type.broadcastable != self.node.outputs[0].type.broadcastable:
             return False
-        return n is self.node or (isinstance(n.op, Elemwise) and any(self.row_shaped(i) for i in n.inputs))
+        if v not in self.shaped:
+            self.shaped[v] = n is self.node or (isinstance(n.op, Elemwise) and
+                                                any(self.row_shaped(i, depth + 1) for i in n.inputs))
+        return self.shaped[v]
 
     def shape_of_rows(self):
         if self.model is None:
             self.model = self.rows()
         return self.model
 
-    def __call__(self, v):
+    def __call__(self, v, depth=0):
         """``v`` without the dependence, or None."""
+        if v not in self.done:
+            self.done[v] = self.rewritten(v, depth) if depth <= self._DEEP else None
+        return self.done[v]
+
+    def rewritten(self, v, depth):
         if not self.depends(v):
             return v
         n = v.owner
@@ -303,7 +323,7 @@ class _Apart(object):
         if isinstance(n.op, T.ShapeFloat) and self.row_shaped(n.inputs[0]):
             return n.op(self.shape_of_rows())
         if isinstance(n.op, Elemwise) and isinstance(n.op.scalar_op, scal.Second):
-            value = self(n.inputs[1])
+            value = self(n.inputs[1], depth + 1)
             if value is None:
                 return None
             if not self.depends(n.inputs[0]):
@@ -314,9 +334,11 @@ class _Apart(object):
                 return None
             return n.op.make_node(model, value).outputs[0]
         if isinstance(n.op, (Elemwise, DimShuffle)) and not getattr(n.op, "inplace_pattern", None):
-            ins = [self(i) for i in n.inputs]
-            if any(i is None for i in ins):
-                return None
+            ins = []
+            for i in n.inputs:
+                ins.append(self(i, depth + 1))
+                if ins[-1] is None:
+                    return None
             return n.op.make_node(*ins).outputs[v.index]
         return None
 
@@ -333,14 +355,18 @@ def _one_value(g):
     return v if isinstance(v.type, HipArrayType) else g
 
 
-def _fuse_layer_normalization(fgraph, node):
+def _places(fgraph):
+    return dict((n, k) for k, n in enumerate(fgraph.toposort()))
+
+
+def _fuse_layer_normalization(fgraph, node, order):
     x, dy, mean, invstd = node.inputs[:4]
     fwd = mean.owner
     if fwd is None or not isinstance(fwd.op, HipLayerNormalization) or [mean, invstd] != list(fwd.outputs[1:]):
         return 0
     if fwd.inputs[0] is not x or list(fwd.inputs[1:2]) != list(node.inputs[4:5]) or len(fwd.inputs) - 1 != node.op.n_params:
         return 0
-    dy = _Apart(fwd, lambda: x)(dy)
+    dy = _Apart(fwd, lambda: x, order)(dy)
     if dy is None:
         return 0
     new = HipLayerNormalizationTrain(fwd.op.epsilon, node.op.n_params).make_node(x, dy, *fwd.inputs[1:])
@@ -357,11 +383,14 @@ def fuse_known_gradients(fgraph):
     a weighted sum or mean of losses, not a function such as a ratio of probabilities; of layer normalisation a gradient
     that is an argument."""
     count = 0
-    for node in fgraph.toposort():
+    order = _places(fgraph)
+    for node in list(order):
         if node not in fgraph.apply_nodes:
             continue
         if isinstance(node.op, HipLayerNormalizationGrad):
-            count += _fuse_layer_normalization(fgraph, node)
+            if _fuse_layer_normalization(fgraph, node, order):
+                order = _places(fgraph)      # what read the result may now stand behind more than it did
+                count += 1
             continue
         if isinstance(node.op, HipTokenLogProbsGrad):
             if node.op.given[2]:
@@ -386,7 +415,7 @@ def fuse_known_gradients(fgraph):
         n = new_op.n_forward
         if fwd.op.temperature != node.op.temperature or list(fwd.inputs) != list(node.inputs[:n]):
             continue
-        apart = _Apart(fwd, rows)
+        apart = _Apart(fwd, rows, order)
         gs = [apart(g) for g in node.inputs[first:]]
         if any(g is None for g in gs):
             continue
@@ -397,6 +426,7 @@ def fuse_known_gradients(fgraph):
         fgraph.replace(dx, new.outputs[-1])
         for o, no in zip(fwd.outputs, new.outputs):
             fgraph.replace(o, no)
+        order = _places(fgraph)
         count += 1
     return count
 
