@@ -288,8 +288,9 @@ int thx_layernorm_train_call(const thx_array* x, const thx_array* dy, const thx_
 
 /* p = softmax(logits / temperature) per row; log_prob = log p[token] (0 where token < 0, NaN where token >= cols),
  * entropy = -sum p log p, the n_top largest log p and their columns (int64; of equal logits the lowest column first,
- * NaN as the largest), stats [rows..., 2] = largest logit m and log2(sum exp((logits - m) / temperature)).  A row of
- * nothing but -infinity: log probabilities -infinity, entropy 0.  tokens: int32 or int64.  n_top 0: top_* null. */
+ * NaN as the largest), stats [rows..., 2] = largest logit m and log2(sum exp((logits - m) / temperature)), for float16
+ * logits relative to a rounding of m, the same in the gradient call at the same temperature (less than half a unit off).
+ * A row of nothing but -infinity: log probabilities -infinity, entropy 0.  tokens: int32 or int64.  n_top 0: top_* null. */
 int thx_token_logprob_workspace(const thx_array* logits, int n_top, size_t* nbytes);
 int thx_token_logprob_call(const thx_array* logits, const thx_array* tokens, double temperature, int n_top,
                            const thx_array* log_prob, const thx_array* entropy, const thx_array* top_log_probs,

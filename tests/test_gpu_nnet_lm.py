@@ -28,8 +28,9 @@ def chain(cols, rows=0):
     return 26 + cols / 64 + rows
 
 
-def close(got, ref, scale, n, what, acc):
-    """``acc``: the type the result was computed in."""
+def close(got, ref, scale, n, what, acc, flush=0.0):
+    """``acc``: the type the result was computed in; ``flush``: what a result may lack where an exponential on the way to
+    it lies below the smallest normal number of that type."""
     got = np.asarray(got)
     fin = np.isfinite(ref)
     assert got.shape == ref.shape, (what, got.shape, ref.shape)
@@ -42,7 +43,7 @@ def close(got, ref, scale, n, what, acc):
     assert (np.abs(g[over]) >= float(info.max)).all(), what
     fin &= ~over
     tol = (float(info.eps) / 2 * np.abs(ref) + float(info.smallest_subnormal) / 2 +
-           n * float(np.finfo(acc).eps) / 2 * np.broadcast_to(scale, ref.shape))
+           n * float(np.finfo(acc).eps) / 2 * np.broadcast_to(scale, ref.shape) + flush)
     with np.errstate(invalid="ignore"):
         bad = fin & ~(np.abs(g - ref) <= tol)
     assert not bad.any(), "%s: %d of %d values, first at %s: got %r, expected %r within %r" % (
@@ -248,7 +249,7 @@ def check_lp(x, tokens, temperature=1.0, n_top=0, w=None, u=None, c=None, dev=No
         check_lp_call(x, tokens, temperature, n_top, given, [v for v in (w, u, c) if v is not None], dev, ref, fuse, what)
 
 
-def check_lp_call(x, tokens, temperature, n_top, given, cotangents, dev, ref, fuse, what):
+def check_lp_call(x, tokens, temperature, n_top, given, cotangents, dev, ref, fuse, what, flush=0.0):
     f = lp_function(str(x.dtype), str(tokens.dtype), x.ndim, n_top, temperature, given, fuse)
     assert any(type(n.op).__name__ == "HipTokenLogProbsTrain" for n in f.toposort()) == fuse
     args = [x, tokens] + cotangents
@@ -265,7 +266,7 @@ def check_lp_call(x, tokens, temperature, n_top, given, cotangents, dev, ref, fu
         close(got[2], *ref["top"], n, what + " top_log_probs", acc)
     if any(given):
         assert got[-1].dtype == x.dtype
-        close(got[-1], *ref["dx"], n, what + " dlogits", acc)
+        close(got[-1], *ref["dx"], n, what + " dlogits", acc, flush)
 
 
 def check_kd(x, teacher, ids, temperature=1.0, g=None, dev=None, what=""):
@@ -274,7 +275,7 @@ def check_kd(x, teacher, ids, temperature=1.0, g=None, dev=None, what=""):
         check_kd_call(x, teacher, ids, temperature, g, dev, ref, fuse, what)
 
 
-def check_kd_call(x, teacher, ids, temperature, g, dev, ref, fuse, what):
+def check_kd_call(x, teacher, ids, temperature, g, dev, ref, fuse, what, flush=0.0):
     f = kd_function(str(x.dtype), str(teacher.dtype), str(ids.dtype), x.ndim, temperature, g is not None, fuse)
     assert any(type(n.op).__name__ == "HipTopKDistillationTrain" for n in f.toposort()) == fuse
     args = [x, teacher, ids] + ([g] if g is not None else [])
@@ -286,7 +287,7 @@ def check_kd_call(x, teacher, ids, temperature, g, dev, ref, fuse, what):
     close(got[0], *ref["loss"], n, what + " loss", acc)
     if g is not None:
         assert got[1].dtype == x.dtype
-        close(got[1], *ref["dx"], n, what + " dlogits", acc)
+        close(got[1], *ref["dx"], n, what + " dlogits", acc, flush)
 
 
 def logits(rng, shape, dtype, spread=3.0):
@@ -546,6 +547,63 @@ def test_large_logits_keep_their_digits():
     x = logits(rng, (3, 700), "float16")
     for t in (1e-3, 50.0):
         check_lp(x, rng.integers(0, 700, 3), n_top=5, temperature=t, w=np.ones(3, "float32"), what="temperature %g" % t)
+
+
+def beside_largest(x):
+    """The differences to the largest of each row, in float64."""
+    x = x.astype("float64")
+    m = x.max(-1, keepdims=True)
+    return x - np.where(np.isfinite(m), m, 0.0)
+
+
+@pytest.mark.parametrize("temperature", [1e-6, 1e-5, 1e-4, 5.6e-3, 5.7e-3])
+@pytest.mark.parametrize("dtype", ["float16", "float32", "float64"])
+def test_large_logits_at_low_temperatures(dtype, temperature):
+    """The largest logit's probability is no smaller than 1 / columns, however large logit / temperature is.  Gradients
+    are weighted so that the results are of order 1.
+
+    Of exponentials below the smallest normal number (2^-126; 2^-1022) the device's single precision gives 0 and the double
+    precision fewer digits, so a probability may be off by that number, and the gradient by that times what p is multiplied
+    with, (w + sum c + u (ln p + H)) / temperature: weights over temperature of at most 5 each, 5 + 5 * 5 of them, ln p
+    down to -89 (-709), H up to ln 20001 < 10.  Distillation: g * temperature, at most 5, times p and q."""
+    rng = np.random.default_rng(16)
+    acc, lowest = acc_of(dtype), float(np.finfo("float16").min)
+    tiny = float(np.finfo(acc).tiny)
+    flush = tiny * (5 + 5 * 5 + 5 * (-np.log(tiny) + 10))
+    for V in (700, 20001):
+        x = np.full((10, V), 10.0)
+        x[0, :2] = 8000, 7000
+        x[1] = 65504 - 32 * rng.integers(0, 100, V)
+        x[2] = lowest
+        x[3] = lowest
+        x[3, ::3] = -INF
+        x[4] = -lowest
+        x[5] = temperature * 3 * rng.standard_normal(V)         # probabilities of many columns
+        x[6] = 3 * rng.standard_normal(V)
+        x[7] = lowest
+        x[7, 5:9] = -8000
+        x[8, [3, 600, V - 1]] = 30000, 30000, 60000
+        x[9] = 10000
+        x[9, 1::2] = 9992
+        x = x.astype(dtype)
+        tokens = rng.integers(0, V, 10)
+        tokens[[0, 5]] = 0, V - 1
+        w, u = [(temperature * rng.standard_normal(10)).astype(acc) for _ in range(2)]
+        c = (temperature * rng.standard_normal((10, 5))).astype(acc)
+        what = "%d columns" % V
+        # logits / temperature would carry a rounding of its own size; of the differences here the plain forms get all digits
+        far = beside_largest(x)
+        ref = lp_ref(far, tokens, temperature, 5, w, u, c)
+        check_lp_call(x, tokens, temperature, 5, (True,) * 3, [w, u, c], None, ref, False, what, flush)
+        ref = lp_ref(far, tokens, temperature, w=w, u=u)
+        for fuse in (True, False):
+            check_lp_call(x, tokens, temperature, 0, (True, True, False), [w, u], None, ref, fuse, what, flush)
+        teacher, ids = x[:, :6].copy(), rng.integers(0, V, (10, 6))
+        ids[:, 0] = np.argmax(x, axis=1)
+        g = (rng.standard_normal(10) / temperature).astype(acc)
+        ref = kd_ref(far, beside_largest(teacher), ids, temperature, g)
+        for fuse in (True, False):
+            check_kd_call(x, teacher, ids, temperature, g, None, ref, fuse, what, 10 * tiny)
 
 
 def test_no_rows():

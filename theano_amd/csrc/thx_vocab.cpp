@@ -3,6 +3,8 @@
 //
 // Everything is computed in binary logarithms: with c = log2(e) / temperature, s_j = c * x_j and the row's largest
 // logit m, S = sum_j 2^(s_j - c m), so log2 p_j = (s_j - c m) - log2 S.  A row keeps (m, log2 S).
+#include <type_traits>
+
 #include "thx_rows.h"
 #include "thx_rows_device.h"
 
@@ -24,20 +26,29 @@ THX_DEV A product(A a, A b) {
   return a * b;
 }
 
-// c * (x - m).  Half precision: one fused multiply-add against the rounded product c * m, which is the same number
-// wherever the row is read, so that its rounding changes no probability; the products of single precision can overflow
-// (a mask of the type's lowest value), their difference is taken first.
-THX_DEV float scaled(thx_f16 x, float m, float c) { return __builtin_fmaf((float)x, c, -product(m, c)); }
-THX_DEV float scaled(float x, float m, float c) { return (x - m) * c; }
-THX_DEV double scaled(double x, double m, double c) { return (x - m) * c; }
-
-// log p in natural units.  In single and double precision not by way of the binary logarithm, whose factor of 1.44 would
-// carry a mask of the type's lowest value beyond the type's range.
-THX_DEV float log_prob(thx_f16 x, float m, float c, float, float ls) { return (scaled(x, m, c) - ls) * (float)kLn2; }
-THX_DEV float log_prob(float x, float m, float, float inv_t, float ls) { return (x - m) * inv_t - ls * (float)kLn2; }
-THX_DEV double log_prob(double x, double m, double, double inv_t, double ls) { return (x - m) * inv_t - ls * kLn2; }
-
 template <class A> THX_DEV A neg_inf() { return -(A)INFINITY; }
+
+// The exponents c * (x - m).  FUSED, half precision at ordinary temperatures: one fused multiply-add against the product
+// c * m, which is rounded, but to the same number wherever the row is read, so that it shifts all exponents of a row and
+// their log2 S alike.  That product has to stay below 2^24 for any logit, which keeps the shift within half a unit; at
+// temperatures under 0.0057 it need not, and the shift can pass the exponents that a float has (a largest logit of 10000
+// at 1e-6: 2^368 in place of 2^0).  There, and in single and double precision, whose products can overflow as well (a mask
+// of the type's lowest value), the difference is taken first.  For half precision that is two operations more to an element:
+// 8192 rows of 50257 with their gradient 366 us in place of 346.
+template <class T, bool FUSED = false>
+struct Exponents {
+  typedef typename AccOf<T>::type A;
+  A c;  // log2(e) / temperature
+  // What the exponents of a row are taken against, 0 while m is -infinity.
+  THX_DEV A reference(A m) const { return m == neg_inf<A>() ? (A)0 : FUSED ? product(m, c) : m; }
+  THX_DEV A of(A x, A ref) const { return FUSED ? __builtin_fmaf(x, c, -ref) : (x - ref) * c; }
+  THX_DEV A between(A ref, A other) const { return FUSED ? ref - other : (ref - other) * c; }  // references
+  // log p in natural units.  Where the difference comes first not by way of the binary logarithm, whose factor of 1.44
+  // would carry a mask of the type's lowest value beyond the type's range.
+  THX_DEV A log_prob(A x, A m, A inv_t, A ls) const {
+    return FUSED ? (of(x, product(m, c)) - ls) * (A)kLn2 : (x - m) * inv_t - ls * (A)kLn2;
+  }
+};
 
 // One value per row or per (row, entry) whose type is not worth a kernel of its own.
 THX_DEV int64_t load_index(const void* p, int is64, int64_t i) { return is64 ? ((const int64_t*)p)[i] : (int64_t)((const int*)p)[i]; }
@@ -80,56 +91,53 @@ template <class Key> THX_DEV int64_t key_column(Key k) { return (int64_t)(0xffff
 // ---- one wave over a part of a row ----------------------------------------------------------------------------------
 //
 // A part of a row is read once, 64 lanes x kUnroll vectors of 16 bytes at a time.  Each lane keeps the largest logit m
-// of its columns and the sums s = sum 2^d and w = sum d 2^d with d = scaled(x, m); they are rescaled when m grows, which
+// of its columns and the sums s = sum 2^d and w = sum d 2^d of the exponents d against m; they are rescaled when m grows, which
 // soon happens rarely.  While m is -infinity the exponents are taken against 0: all of them are 0, or NaN, which stays.
 
 constexpr int kUnroll = 4;
 constexpr int kWaves = 4;     // waves of a block; each works alone
 constexpr int kList = 512;    // candidates a wave can hold
 
-template <class T, bool ENT>
+template <class T, bool ENT, bool FUSED = false>
 struct LaneSums {
   typedef typename AccOf<T>::type A;
+  typedef Exponents<T, FUSED> Ex;
   A m, s, w;
-  A ref;  // what the exponents are taken against: m * c for half precision, else m; 0 while m is -infinity
+  A ref;  // what the exponents are taken against
   THX_DEV void init() {
     m = neg_inf<A>();
     s = w = ref = 0;
   }
-  THX_DEV A exponent(A x, A c) const {
-    if constexpr (sizeof(T) == 2) return __builtin_fmaf(x, c, -ref);
-    else return (x - ref) * c;
-  }
   // d 2^d is 0 where 2^d is, for d = -infinity as well
   THX_DEV static float bounded(float d) { return __builtin_fmaxf(d, -30000.0f); }
   THX_DEV static double bounded(double d) { return __builtin_fmax(d, -30000.0); }
-  THX_DEV void raise(A to, A c) {  // to > m
+  THX_DEV void raise(A to, const Ex& ex) {  // to > m
     const A old = ref;
-    ref = sizeof(T) == 2 ? product(to, c) : to;
+    ref = ex.reference(to);
     // between the references as they were rounded, not between the logits
-    const A d = m == neg_inf<A>() ? neg_inf<A>() : sizeof(T) == 2 ? old - ref : (old - ref) * c, k = acc_exp2(d);
+    const A d = m == neg_inf<A>() ? neg_inf<A>() : ex.between(old, ref), k = acc_exp2(d);
     m = to;
     if (ENT) w = k * (w + bounded(d) * s);
     s *= k;
   }
-  THX_DEV void add(A x, A c) {
-    const A d = exponent(x, c), e = acc_exp2(d);
+  THX_DEV void add(A x, const Ex& ex) {
+    const A d = ex.of(x, ref), e = acc_exp2(d);
     s += e;
     if (ENT) w += e * bounded(d);
   }
   // Takes in the sums of other columns.
-  THX_DEV void join(A om, A os, A ow, A c) {
+  THX_DEV void join(A om, A os, A ow, const Ex& ex) {
     LaneSums o;
     o.m = om, o.s = os, o.w = ow;
-    o.ref = om == neg_inf<A>() ? (A)0 : (sizeof(T) == 2 ? product(om, c) : om);
-    if (om > m) raise(om, c);
-    else if (m > om) o.raise(m, c);
+    o.ref = ex.reference(om);
+    if (om > m) raise(om, ex);
+    else if (m > om) o.raise(m, ex);
     s += o.s;
     if (ENT) w += o.w;
   }
-  THX_DEV void join_lanes(A c) {
+  THX_DEV void join_lanes(const Ex& ex) {
     const A all = wave_largest(m);
-    if (all > m) raise(all, c);
+    if (all > m) raise(all, ex);
     s = lanes_sum<64>(s);
     if (ENT) w = lanes_sum<64>(w);
   }
@@ -258,9 +266,9 @@ struct Best {
 };
 
 // The sums of the vectors [lo, hi) of a row, and its best vectors.
-template <class T, bool ENT, bool TOP>
-THX_DEV void read_part(const T* x, int64_t cols, int64_t lo, int64_t hi, typename AccOf<T>::type c, LaneSums<T, ENT>& sum,
-                       Best<T>& best) {
+template <class T, bool ENT, bool TOP, bool FUSED>
+THX_DEV void read_part(const T* x, int64_t cols, int64_t lo, int64_t hi, const Exponents<T, FUSED>& ex,
+                       LaneSums<T, ENT, FUSED>& sum, Best<T>& best) {
   typedef typename AccOf<T>::type A;
   constexpr int V = Width<T>::value;
   const int lane = threadIdx.x & 63;
@@ -290,11 +298,11 @@ THX_DEV void read_part(const T* x, int64_t cols, int64_t lo, int64_t hi, typenam
     A m = vm[0];
 #pragma unroll
     for (int u = 1; u < kUnroll; ++u) m = m > vm[u] ? m : vm[u];
-    if (m > sum.m) sum.raise(m, c);
+    if (m > sum.m) sum.raise(m, ex);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) sum.add((A)v[u].v[e], c);
+      for (int e = 0; e < V; ++e) sum.add((A)v[u].v[e], ex);
       // one vector after the other: with 32 exponentials at once the half-precision kernel takes 181 registers, not 116
       if constexpr (TOP && sizeof(T) < 8) asm volatile("" : "+v"(sum.s), "+v"(sum.w));
     }
@@ -345,9 +353,9 @@ struct LpRow {  // what lp_forward needs besides the logits
 };
 
 // The best columns out of the best vectors (in best.list, falling), and everything else of the row; `sum` joined.
-template <class T, bool TOP>
-THX_DEV void finish(const LpRow<T>& q, const T* x, int64_t cols, int64_t r, typename AccOf<T>::type c,
-                    const LaneSums<T, true>& sum, Best<T>& best) {
+template <class T, bool TOP, bool FUSED>
+THX_DEV void finish(const LpRow<T>& q, const T* x, int64_t cols, int64_t r, const Exponents<T, FUSED>& ex,
+                    const LaneSums<T, true, FUSED>& sum, Best<T>& best) {
   typedef typename AccOf<T>::type A;
   typedef typename Order<T>::Key Key;
   constexpr int V = Width<T>::value;
@@ -358,7 +366,7 @@ THX_DEV void finish(const LpRow<T>& q, const T* x, int64_t cols, int64_t r, type
     const int64_t t = load_index(q.tokens, q.t64, r * q.ts);
     A lp = 0;
     if (t >= cols) lp = (A)NAN;
-    else if (t >= 0) lp = none ? neg_inf<A>() : log_prob(x[t], sum.m, c, q.inv_t, ls);
+    else if (t >= 0) lp = none ? neg_inf<A>() : ex.log_prob((A)x[t], sum.m, q.inv_t, ls);
     q.o.log_prob[r] = lp;
     q.o.entropy[r] = none ? (A)0 : (ls - sum.w / sum.s) * (A)kLn2;
     q.o.stats[2 * r] = sum.m;
@@ -388,7 +396,7 @@ THX_DEV void finish(const LpRow<T>& q, const T* x, int64_t cols, int64_t r, type
     if (lane < k) {
       const int64_t j = key_column(best.list[lane]);
       q.o.top_at[r * k + lane] = j;
-      q.o.top[r * k + lane] = none ? neg_inf<A>() : log_prob(x[j], sum.m, c, q.inv_t, ls);
+      q.o.top[r * k + lane] = none ? neg_inf<A>() : ex.log_prob((A)x[j], sum.m, q.inv_t, ls);
     }
   }
 }
@@ -413,23 +421,24 @@ THX_DEV Entry<A> load_entry(const Teacher<A>& t, int64_t r, int k) {
 // An entry into the teacher's sums: nothing where it stands for no token, NaN where it names one that is not there, which
 // makes the row's loss and gradient NaN.
 template <class A>
-THX_DEV void take_entry(const Entry<A>& e, int64_t cols, A c, LaneSums<A, false>& ts) {
+THX_DEV void take_entry(const Entry<A>& e, int64_t cols, const Exponents<A>& ex, LaneSums<A, false>& ts) {
   if (e.id < 0) return;
-  if (e.logit > ts.m) ts.raise(e.logit, c);
-  ts.add(e.logit, c);
+  if (e.logit > ts.m) ts.raise(e.logit, ex);
+  ts.add(e.logit, ex);
   if (e.id >= cols) ts.s = (A)NAN;
 }
 
 // q (log q - log p) of an entry, `at` being its column's logit; 0 where q is, or where it stands for no token.
-template <class T, class A>
-THX_DEV A entry_loss(const KdRow<T>& q, const Entry<A>& e, T at, int64_t cols, A c, const LaneSums<T, false>& sum, A ls, A tm,
-                     A tls) {
+template <class T, class A, bool FUSED>
+THX_DEV A entry_loss(const KdRow<T>& q, const Entry<A>& e, T at, int64_t cols, const Exponents<T, FUSED>& ex,
+                     const LaneSums<T, false, FUSED>& sum, A ls, A tm, A tls) {
+  const Exponents<A> tex = {ex.c};
   if (e.id < 0 || (tm == neg_inf<A>() && tls == neg_inf<A>())) return 0;
-  const A p = acc_exp2((e.logit - tm) * c - tls);
+  const A p = acc_exp2(tex.of(e.logit, tm) - tls);
   if (p == (A)0) return 0;
   if (e.id >= cols) return (A)NAN;
-  const A lp = sum.nothing_left() ? neg_inf<A>() : log_prob(at, sum.m, c, q.inv_t, ls);
-  return p * (log_prob(e.logit, tm, c, q.inv_t, tls) - lp);
+  const A lp = sum.nothing_left() ? neg_inf<A>() : ex.log_prob((A)at, sum.m, q.inv_t, ls);
+  return p * (tex.log_prob(e.logit, tm, q.inv_t, tls) - lp);
 }
 
 // The logit of an entry's column, anything where it has none.
@@ -438,22 +447,23 @@ THX_DEV T entry_at(const Entry<A>& e, const T* x, int64_t cols) {
   return e.id >= 0 && e.id < cols ? x[e.id] : (T)0;
 }
 
-template <class T>
-THX_DEV void finish(const KdRow<T>& q, const T* x, int64_t cols, int64_t r, typename AccOf<T>::type c,
-                    const LaneSums<T, false>& sum) {
+template <class T, bool FUSED>
+THX_DEV void finish(const KdRow<T>& q, const T* x, int64_t cols, int64_t r, const Exponents<T, FUSED>& ex,
+                    const LaneSums<T, false, FUSED>& sum) {
   typedef typename AccOf<T>::type A;
   const Teacher<A>& t = q.t;
   const int lane = threadIdx.x & 63;
   const A ls = sum.log2_sum();
   LaneSums<A, false> ts;  // the teacher's side: entries as single or double precision
+  const Exponents<A> tex = {ex.c};
   ts.init();
-  for (int k = lane; k < t.n; k += 64) take_entry(load_entry(t, r, k), cols, c, ts);
-  ts.join_lanes(c);
+  for (int k = lane; k < t.n; k += 64) take_entry(load_entry(t, r, k), cols, tex, ts);
+  ts.join_lanes(tex);
   const A tls = ts.log2_sum();
   A loss = 0;
   for (int k = lane; k < t.n; k += 64) {
     const Entry<A> e = load_entry(t, r, k);
-    loss += entry_loss(q, e, entry_at(e, x, cols), cols, c, sum, ls, ts.m, tls);
+    loss += entry_loss(q, e, entry_at(e, x, cols), cols, ex, sum, ls, ts.m, tls);
   }
   loss = lanes_sum<64>(loss);
   if (sum.s != sum.s) loss = sum.s;
@@ -470,20 +480,20 @@ THX_DEV void finish(const KdRow<T>& q, const T* x, int64_t cols, int64_t r, type
 
 // The rows of a call and how they are cut: `parts` waves to a row, `per` vectors to a part.  A row of several parts leaves
 // its sums in partial[row][part][3] and its best vectors (k of them, 0 for none) in lists[row][part][k].
-template <class T>
+template <class T, bool FUSED>
 struct Cut {
   typedef typename AccOf<T>::type A;
   const T* x;
   int64_t xs, rows, cols;
   int64_t per;
   int parts;
-  A c;
+  Exponents<T, FUSED> ex;
   A* partial;
   typename Order<T>::Key* lists;
 };
 
-template <class T, bool TOP, class Row, bool ENT>
-__global__ void __launch_bounds__(64 * kWaves) vocab_read(Cut<T> q, Row row) {
+template <class T, bool TOP, class Row, bool ENT, bool FUSED>
+__global__ void __launch_bounds__(64 * kWaves) vocab_read(Cut<T, FUSED> q, Row row) {
   typedef typename Order<T>::Key Key;
   constexpr int V = Width<T>::value;
   __shared__ Key lists[TOP ? kWaves * kList : 1];
@@ -493,18 +503,18 @@ __global__ void __launch_bounds__(64 * kWaves) vocab_read(Cut<T> q, Row row) {
     const int64_t r = unit / q.parts, part = unit - r * q.parts;
     const T* x = q.x + r * q.xs;
     const int64_t lo = part * q.per, hi = lo + q.per < vectors ? lo + q.per : vectors;
-    LaneSums<T, ENT> sum;
+    LaneSums<T, ENT, FUSED> sum;
     Best<T> best;
     int k = 0;
     if constexpr (TOP) {
       k = row.n_top;
       best.init(lists + wave * kList, k);
     }
-    read_part<T, ENT, TOP>(x, q.cols, lo, hi, q.c, sum, best);
-    sum.join_lanes(q.c);
+    read_part<T, ENT, TOP>(x, q.cols, lo, hi, q.ex, sum, best);
+    sum.join_lanes(q.ex);
     if (q.parts == 1) {
-      if constexpr (ENT) finish<T, TOP>(row, x, q.cols, r, q.c, sum, best);
-      else finish<T>(row, x, q.cols, r, q.c, sum);
+      if constexpr (ENT) finish<T, TOP>(row, x, q.cols, r, q.ex, sum, best);
+      else finish<T>(row, x, q.cols, r, q.ex, sum);
       wave_fence();
       continue;
     }
@@ -518,20 +528,20 @@ __global__ void __launch_bounds__(64 * kWaves) vocab_read(Cut<T> q, Row row) {
 }
 
 // One wave per row over its parts (at most 64: one to a lane).
-template <class T, bool TOP, class Row, bool ENT>
-__global__ void __launch_bounds__(64) vocab_join(Cut<T> q, Row row) {
+template <class T, bool TOP, class Row, bool ENT, bool FUSED>
+__global__ void __launch_bounds__(64) vocab_join(Cut<T, FUSED> q, Row row) {
   typedef typename AccOf<T>::type A;
   typedef typename Order<T>::Key Key;
   __shared__ Key lists[TOP ? kList : 1];
   const int lane = threadIdx.x;
   for (int64_t r = blockIdx.x; r < q.rows; r += gridDim.x) {
-    LaneSums<T, ENT> sum;
+    LaneSums<T, ENT, FUSED> sum;
     sum.init();
     if (lane < q.parts) {
       const auto* p = q.partial + (r * q.parts + lane) * 3;
-      sum.join(p[0], p[1], p[2], q.c);
+      sum.join(p[0], p[1], p[2], q.ex);
     }
-    sum.join_lanes(q.c);
+    sum.join_lanes(q.ex);
     const T* x = q.x + r * q.xs;
     if constexpr (ENT) {
       Best<T> best;
@@ -567,9 +577,9 @@ __global__ void __launch_bounds__(64) vocab_join(Cut<T> q, Row row) {
         best.sort(k);
         wave_fence();
       }
-      finish<T, TOP>(row, x, q.cols, r, q.c, sum, best);
+      finish<T, TOP>(row, x, q.cols, r, q.ex, sum, best);
     } else {
-      finish<T>(row, x, q.cols, r, q.c, sum);
+      finish<T>(row, x, q.cols, r, q.ex, sum);
     }
     wave_fence();
   }
@@ -578,7 +588,7 @@ __global__ void __launch_bounds__(64) vocab_join(Cut<T> q, Row row) {
 // ---- gradient ------------------------------------------------------------------------------------------------------------
 //
 // dx_j = p_j (a + b log2 p_j) + sum_k v_k [j = id_k] is the gradient of every function of the log probabilities above.
-// With d = scaled(x_j, m) and p_j = 2^d / S it is 2^d (a' + b' d) with a' = (a - b log2 S) / S and b' = b / S: one
+// With the exponent d of x_j against m and p_j = 2^d / S it is 2^d (a' + b' d) with a' = (a - b log2 S) / S and b' = b / S: one
 // exponential and one rounding of the row's statistics per element.  The columns of the list are few; their elements are
 // written once more, each by the thread of the entry that names the column first, from the sum of all entries that do.
 
@@ -642,29 +652,29 @@ struct KdGrad {
   }
 };
 
-template <class T>
+template <class T, bool FUSED>
 struct GradCut {
   typedef typename AccOf<T>::type A;
   const T* x;
   int64_t xs, rows, cols;
   int64_t per;  // vectors of a segment
   int segs;     // segments of a row
-  A c;
+  Exponents<T, FUSED> ex;
   T* dx;
   bool nt;      // dx is streamed past the caches
 };
 
 
 // The slope of a row's elements.
-template <class T>
+template <class T, bool FUSED>
 struct RowSlope {
   typedef typename AccOf<T>::type A;
-  LaneSums<T, false> at;
-  A a, b, c;
+  Exponents<T, FUSED> ex;
+  A ref, a, b;
   bool none;
-  THX_DEV RowSlope(const Slope<A>& s, A c_) : c(c_) {
+  THX_DEV RowSlope(const Slope<A>& s, const Exponents<T, FUSED>& ex_) : ex(ex_) {
     none = s.m == neg_inf<A>() && s.ls == neg_inf<A>();
-    at.ref = none ? (A)0 : sizeof(T) == 2 ? product(s.m, c) : s.m;
+    ref = ex.reference(s.m);
     const A inv = none ? (A)0 : acc_exp2(-s.ls);
     a = none ? (A)0 : (s.a - s.b * s.ls) * inv;
     b = s.b * inv;
@@ -672,7 +682,7 @@ struct RowSlope {
   THX_DEV A operator()(T v) const { return b == (A)0 ? of<false>(v) : of<true>(v); }
   template <bool B>
   THX_DEV A of(T v) const {
-    const A d = at.exponent((A)v, c), e = acc_exp2(d);
+    const A d = ex.of((A)v, ref), e = acc_exp2(d);
     return B ? e * (a + b * LaneSums<T, false>::bounded(d)) : e * a;
   }
   // In place, over N vectors; whether there is a b is the same for the whole row.
@@ -699,8 +709,8 @@ struct RowSlope {
 
 // Element j of a row's gradient, which entry k of the list names, written over; behind a barrier.  The first entry of a
 // column writes for all that name it.
-template <class T, class A>
-THX_DEV void write_entry(const RowSlope<T>& slope, T at, T* dx, const int* id, const A* val, int n, int k, int j) {
+template <class T, class A, bool FUSED>
+THX_DEV void write_entry(const RowSlope<T, FUSED>& slope, T at, T* dx, const int* id, const A* val, int n, int k, int j) {
   A v = 0;
   int before = 0, i = 0;
   for (; i + 4 <= n; i += 4) {  // four at a time: each is a wait for LDS
@@ -720,8 +730,8 @@ THX_DEV void write_entry(const RowSlope<T>& slope, T at, T* dx, const int* id, c
 }
 
 // All elements of columns [first, last) that the list names.
-template <class T, class A>
-THX_DEV void write_entries(const RowSlope<T>& slope, const T* x, T* dx, const int* id, const A* val, int n, int64_t first,
+template <class T, class A, bool FUSED>
+THX_DEV void write_entries(const RowSlope<T, FUSED>& slope, const T* x, T* dx, const int* id, const A* val, int n, int64_t first,
                            int64_t last, int from = 0) {
   for (int k = from + threadIdx.x; k < n; k += blockDim.x) {
     const int j = id[k];
@@ -729,8 +739,8 @@ THX_DEV void write_entries(const RowSlope<T>& slope, const T* x, T* dx, const in
   }
 }
 
-template <class T, class Row>
-__global__ void __launch_bounds__(256) vocab_grad(GradCut<T> q, Row row) {
+template <class T, class Row, bool FUSED>
+__global__ void __launch_bounds__(256) vocab_grad(GradCut<T, FUSED> q, Row row) {
   typedef typename AccOf<T>::type A;
   constexpr int V = Width<T>::value;
   __shared__ __align__(16) int id[Row::kEntries];
@@ -740,7 +750,7 @@ __global__ void __launch_bounds__(256) vocab_grad(GradCut<T> q, Row row) {
     const int64_t r = unit / q.segs, seg = unit - r * q.segs;
     const T* x = q.x + r * q.xs;
     T* dx = q.dx + r * q.cols;
-    const RowSlope<T> slope(row.open(r, q.cols, id, val), q.c);
+    const RowSlope<T, FUSED> slope(row.open(r, q.cols, id, val), q.ex);
     const int64_t lo = seg * q.per, hi = lo + q.per < vectors ? lo + q.per : vectors;
     for (int64_t i0 = lo; i0 < hi; i0 += 256 * kUnroll) {
       Vec<T, V> v[kUnroll];
@@ -789,8 +799,8 @@ struct KdTrain {
   A temperature;
 };
 
-template <class T, class Row, int THREADS, int VPT>
-__global__ void __launch_bounds__(THREADS, VPT > 8 && sizeof(T) < 8 ? 4 : 1) vocab_train(GradCut<T> q, Row row) {
+template <class T, class Row, int THREADS, int VPT, bool FUSED>
+__global__ void __launch_bounds__(THREADS, VPT > 8 && sizeof(T) < 8 ? 4 : 1) vocab_train(GradCut<T, FUSED> q, Row row) {
   typedef typename AccOf<T>::type A;
   constexpr int V = Width<T>::value, W = THREADS / 64;
   constexpr bool ENT = Row::kEntropy;
@@ -830,10 +840,10 @@ __global__ void __launch_bounds__(THREADS, VPT > 8 && sizeof(T) < 8 ? 4 : 1) voc
     const bool extra = (int)threadIdx.x < rest;
     const T tail = extra ? x[(int64_t)whole * V + threadIdx.x] : (T)neg_inf<A>();
     if constexpr (!ENT) mine_at = entry_at<T, A>({mine_id, mine_logit}, x, q.cols);
-    LaneSums<T, ENT> sum;
+    LaneSums<T, ENT, FUSED> sum;
     sum.init();
-    if ((A)tail > sum.m) sum.raise((A)tail, q.c);
-    sum.add((A)tail, q.c);
+    if ((A)tail > sum.m) sum.raise((A)tail, q.ex);
+    sum.add((A)tail, q.ex);
 #pragma unroll
     for (int u = 0; u < VPT; u += G) {
       if (u > full) continue;
@@ -843,26 +853,27 @@ __global__ void __launch_bounds__(THREADS, VPT > 8 && sizeof(T) < 8 ? 4 : 1) voc
         const A o = vector_max(v[u + k]);
         m = m > o ? m : o;
       }
-      if (m > sum.m) sum.raise(m, q.c);
+      if (m > sum.m) sum.raise(m, q.ex);
 #pragma unroll
       for (int k = 0; k < G; ++k)
 #pragma unroll
-        for (int e = 0; e < V; ++e) sum.add((A)v[u + k].v[e], q.c);
+        for (int e = 0; e < V; ++e) sum.add((A)v[u + k].v[e], q.ex);
     }
 #pragma unroll
     for (int u = 0; u < VPT; ++u) forget(v[u]);
-    sum.join_lanes(q.c);
+    sum.join_lanes(q.ex);
     if (lane == 0) {
       part[wave][0] = sum.m, part[wave][1] = sum.s;
       if constexpr (ENT) part[wave][2] = sum.w;
     }
     [[maybe_unused]] LaneSums<A, false> ts;
+    [[maybe_unused]] const Exponents<A> tex = {q.ex.c};
     if constexpr (!ENT) {
       ts.init();
-      take_entry({mine_id, mine_logit}, q.cols, q.c, ts);
+      take_entry({mine_id, mine_logit}, q.cols, tex, ts);
       for (int k = threadIdx.x + THREADS; k < row.out.t.n; k += THREADS)
-        take_entry(load_entry(row.out.t, r, k), q.cols, q.c, ts);
-      ts.join_lanes(q.c);
+        take_entry(load_entry(row.out.t, r, k), q.cols, tex, ts);
+      ts.join_lanes(tex);
       if (lane == 0) part[wave][2] = ts.m, part[wave][3] = ts.s;
     }
     __syncthreads();
@@ -870,8 +881,8 @@ __global__ void __launch_bounds__(THREADS, VPT > 8 && sizeof(T) < 8 ? 4 : 1) voc
     if constexpr (!ENT) ts.init();
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      sum.join(part[w][0], part[w][1], ENT ? part[w][2] : (A)0, q.c);
-      if constexpr (!ENT) ts.join(part[w][2], part[w][3], (A)0, q.c);
+      sum.join(part[w][0], part[w][1], ENT ? part[w][2] : (A)0, q.ex);
+      if constexpr (!ENT) ts.join(part[w][2], part[w][3], (A)0, tex);
     }
     const A ls = sum.log2_sum();
     Slope<A> s = {sum.m, ls, (A)0, (A)0};
@@ -890,7 +901,7 @@ __global__ void __launch_bounds__(THREADS, VPT > 8 && sizeof(T) < 8 ? 4 : 1) voc
         val[0] = w * o.inv_t;
         A lp = 0;
         if (t >= q.cols) lp = (A)NAN;
-        else if (t >= 0) lp = sum.nothing_left() ? neg_inf<A>() : log_prob(x[t], sum.m, q.c, o.inv_t, ls);
+        else if (t >= 0) lp = sum.nothing_left() ? neg_inf<A>() : q.ex.log_prob((A)x[t], sum.m, o.inv_t, ls);
         o.o.log_prob[r] = lp;
         o.o.entropy[r] = entropy;
         o.o.stats[2 * r] = sum.m;
@@ -908,7 +919,7 @@ __global__ void __launch_bounds__(THREADS, VPT > 8 && sizeof(T) < 8 ? 4 : 1) voc
         o.stats[4 * r + 3] = tls;
       }
     }
-    const RowSlope<T> slope(s, q.c);
+    const RowSlope<T, FUSED> slope(s, q.ex);
     T* dt = dx + (int)threadIdx.x * V;
 #pragma unroll
     for (int u = 0; u < VPT; ++u) {
@@ -923,8 +934,8 @@ __global__ void __launch_bounds__(THREADS, VPT > 8 && sizeof(T) < 8 ? 4 : 1) voc
       A loss = 0;
       auto put = [&](int k, const Entry<A>& e, T at) {
         id[k] = e.id >= 0 && e.id < q.cols && !ts.nothing_left() ? (int)e.id : -1;
-        val[k] = -gt * acc_exp2((e.logit - ts.m) * q.c - tls);
-        loss += entry_loss(o, e, at, q.cols, q.c, sum, ls, ts.m, tls);
+        val[k] = -gt * acc_exp2(tex.of(e.logit, ts.m) - tls);
+        loss += entry_loss(o, e, at, q.cols, q.ex, sum, ls, ts.m, tls);
       };
       if ((int)threadIdx.x < n) put(threadIdx.x, {mine_id, mine_logit}, mine_at);
       for (int k = threadIdx.x + THREADS; k < n; k += THREADS) {
@@ -981,48 +992,60 @@ std::string plan_of(const char* name, const Rows& x) {
          std::to_string(parts_of(x.rows, ceil_div(x.cols * dtype_size(x.dtype), 16)));
 }
 
-template <class T>
-Cut<T> cut_of(const Rows& x, double temperature, void* ws) {
+// f(T(), whether the exponents are the fused ones) for the type of the logits.
+template <class F>
+int by_type(int x, double temperature, F&& f) {
+  if (x == THX_F16) {
+    // the largest finite half times c below 2^24
+    if (65504.0 * (kLog2E / temperature) < 16777216.0) return f(thx_f16(), std::true_type());
+    return f(thx_f16(), std::false_type());
+  }
+  if (x == THX_F32) return f(thx_f32(), std::false_type());
+  return f(thx_f64(), std::false_type());
+}
+
+template <class T, bool FUSED>
+Cut<T, FUSED> cut_of(const Rows& x, double temperature, void* ws) {
   typedef typename AccOf<T>::type A;
-  Cut<T> q;
+  Cut<T, FUSED> q;
   const int64_t vectors = ceil_div(x.cols, Width<T>::value);
   q.x = (const T*)x.ptr;
   q.xs = x.stride, q.rows = x.rows, q.cols = x.cols;
   q.parts = parts_of(x.rows, vectors);
   q.per = ceil_div(vectors, q.parts);
-  q.c = (A)(kLog2E / temperature);
+  q.ex = {(A)(kLog2E / temperature)};
   q.partial = (A*)ws;
   q.lists = (typename Order<T>::Key*)((char*)ws + ((size_t)x.rows * q.parts * 3 * sizeof(A) + 15) / 16 * 16);
   return q;
 }
 
-template <class T, bool TOP, bool ENT, class Row>
-int launch_forward(Cut<T> q, Row row, const std::string& plan) {
+template <class T, bool TOP, bool ENT, bool FUSED, class Row>
+int launch_forward(Cut<T, FUSED> q, Row row, const std::string& plan) {
   void* args[] = {&q, &row};
   const int64_t units = q.rows * q.parts;
-  int rc = launch_builtin((const void*)&vocab_read<T, TOP, Row, ENT>, plan, dim3(grid_of(ceil_div(units, kWaves))),
+  int rc = launch_builtin((const void*)&vocab_read<T, TOP, Row, ENT, FUSED>, plan, dim3(grid_of(ceil_div(units, kWaves))),
                           dim3(64 * kWaves), args);
   if (rc || q.parts == 1) return rc;
-  return launch_builtin((const void*)&vocab_join<T, TOP, Row, ENT>, plan + "|join", dim3(grid_of(q.rows)), dim3(64), args);
+  return launch_builtin((const void*)&vocab_join<T, TOP, Row, ENT, FUSED>, plan + "|join", dim3(grid_of(q.rows)), dim3(64), args);
 }
 
 // The gradient's segments: 16 blocks to a compute unit where there are too few rows for that, one vector to a thread at
 // least; whole rows else, since every segment reads the row's list again (2048 rows of 32000 floats, 64 entries: 153 us
 // in segments of 4 vectors to a thread, 116 us in two segments a row).
-template <class T, class Row>
+template <class T, bool FUSED, class Row>
 int launch_grad(const Rows& x, double temperature, const Rows& dx, Row row, const std::string& plan) {
   typedef typename AccOf<T>::type A;
-  GradCut<T> q;
+  GradCut<T, FUSED> q;
   const int64_t vectors = ceil_div(x.cols, Width<T>::value);
   q.x = (const T*)x.ptr;
   q.xs = x.stride, q.rows = x.rows, q.cols = x.cols;
   q.segs = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(vectors, 256), ceil_div(16 * compute_units(), x.rows)));
   q.per = ceil_div(vectors, q.segs);
-  q.c = (A)(kLog2E / temperature);
+  q.ex = {(A)(kLog2E / temperature)};
   q.dx = (T*)dx.ptr;
   q.nt = stream_out(x, dx);
   void* args[] = {&q, &row};
-  return launch_builtin((const void*)&vocab_grad<T, Row>, plan, dim3(grid_of(x.rows * q.segs)), dim3(256), args);
+  return launch_builtin((const void*)&vocab_grad<T, Row, FUSED>, plan, dim3(grid_of(x.rows * q.segs)), dim3(256), args);
 }
 
 // The block that holds a row of the one-pass kernel: threads, and vectors to a thread; 0 where none does.  Two blocks of a
@@ -1047,38 +1070,31 @@ std::string held_plan(const char* name, const Rows& x, const Hold& h) {
   return std::string(name) + "|t" + std::to_string(x.dtype) + "|r" + std::to_string(h.threads) + "x" + std::to_string(h.vpt);
 }
 
-template <class T, class Row>
+template <class T, bool FUSED, class Row>
 int launch_train(const Rows& x, double temperature, const Rows& dx, const Hold& h, Row row, const std::string& plan) {
   typedef typename AccOf<T>::type A;
-  GradCut<T> q = {};
+  GradCut<T, FUSED> q = {};
   q.x = (const T*)x.ptr;
   q.xs = x.stride, q.rows = x.rows, q.cols = x.cols;
-  q.c = (A)(kLog2E / temperature);
+  q.ex = {(A)(kLog2E / temperature)};
   q.dx = (T*)dx.ptr;
   q.nt = stream_out(x, dx);
   void* args[] = {&q, &row};
   const void* kernel = nullptr;
   switch (h.threads * 32 + h.vpt) {
-    case 256 * 32 + 1: kernel = (const void*)&vocab_train<T, Row, 256, 1>; break;
-    case 256 * 32 + 2: kernel = (const void*)&vocab_train<T, Row, 256, 2>; break;
-    case 256 * 32 + 4: kernel = (const void*)&vocab_train<T, Row, 256, 4>; break;
-    case 256 * 32 + 8: kernel = (const void*)&vocab_train<T, Row, 256, 8>; break;
-    case 512 * 32 + 8: kernel = (const void*)&vocab_train<T, Row, 512, 8>; break;
-    case 512 * 32 + 16: kernel = (const void*)&vocab_train<T, Row, 512, 16>; break;
+    case 256 * 32 + 1: kernel = (const void*)&vocab_train<T, Row, 256, 1, FUSED>; break;
+    case 256 * 32 + 2: kernel = (const void*)&vocab_train<T, Row, 256, 2, FUSED>; break;
+    case 256 * 32 + 4: kernel = (const void*)&vocab_train<T, Row, 256, 4, FUSED>; break;
+    case 256 * 32 + 8: kernel = (const void*)&vocab_train<T, Row, 256, 8, FUSED>; break;
+    case 512 * 32 + 8: kernel = (const void*)&vocab_train<T, Row, 512, 8, FUSED>; break;
+    case 512 * 32 + 16: kernel = (const void*)&vocab_train<T, Row, 512, 16, FUSED>; break;
     default:
       if constexpr (sizeof(T) < 8)
-        kernel = h.threads == 512  ? (const void*)&vocab_train<T, Row, 512, 20>
-                 : h.vpt == 16 ? (const void*)&vocab_train<T, Row, 1024, 16>
-                               : (const void*)&vocab_train<T, Row, 1024, 20>;
+        kernel = h.threads == 512  ? (const void*)&vocab_train<T, Row, 512, 20, FUSED>
+                 : h.vpt == 16 ? (const void*)&vocab_train<T, Row, 1024, 16, FUSED>
+                               : (const void*)&vocab_train<T, Row, 1024, 20, FUSED>;
   }
   return launch_builtin(kernel, plan, dim3(grid_of(x.rows)), dim3(h.threads), args);
-}
-
-template <class F>
-int by_type(int x, F&& f) {
-  if (x == THX_F16) return f(thx_f16());
-  if (x == THX_F32) return f(thx_f32());
-  return f(thx_f64());
 }
 
 // The logits of a call: checked for type, width and temperature.
@@ -1138,12 +1154,13 @@ int token_logprob(const thx_array* logits, const thx_array* tokens, double tempe
   set_last_plan(plan);
   if (dry || !in[0].rows) return THX_OK;
   if ((rc = ensure_init())) return rc;
-  return by_type(in[0].dtype, [&](auto t) {
+  return by_type(in[0].dtype, temperature, [&](auto t, auto fused) {
     typedef decltype(t) T;
+    constexpr bool FUSED = decltype(fused)::value;
     typedef typename AccOf<T>::type A;
     const LpRow<T> row = {in[1].ptr, in[1].stride, in[1].dtype == THX_I64, n_top, (A)(1.0 / temperature),
                           {(A*)out[0].ptr, (A*)out[1].ptr, (A*)out[3].ptr, (int64_t*)out[4].ptr, (A*)out[2].ptr}};
-    const Cut<T> q = cut_of<T>(in[0], temperature, ws);
+    const Cut<T, FUSED> q = cut_of<T, FUSED>(in[0], temperature, ws);
     return n_top ? launch_forward<T, true, true>(q, row, plan) : launch_forward<T, false, true>(q, row, plan);
   });
 }
@@ -1177,13 +1194,14 @@ int token_logprob_grad(const thx_array* logits, const thx_array* tokens, const t
   set_last_plan(plan);
   if (dry || !in[0].rows) return THX_OK;
   if ((rc = ensure_init())) return rc;
-  return by_type(in[0].dtype, [&](auto t) {
+  return by_type(in[0].dtype, temperature, [&](auto t, auto fused) {
     typedef decltype(t) T;
+    constexpr bool FUSED = decltype(fused)::value;
     typedef typename AccOf<T>::type A;
     const LpGrad<A> q = {in[1].ptr, in[1].stride, in[1].dtype == THX_I64, (const A*)in[2].ptr, in[2].stride, (const A*)in[3].ptr,
                    in[3].stride, (const int64_t*)in[4].ptr, in[4].stride, (int)n_top, (const A*)in[5].ptr, in[5].stride,
                    (const A*)in[6].ptr, in[6].stride, (const A*)in[7].ptr, in[7].stride, (A)(1.0 / temperature)};
-    return launch_grad<T>(in[0], temperature, out, q, plan);
+    return launch_grad<T, FUSED>(in[0], temperature, out, q, plan);
   });
 }
 
@@ -1226,12 +1244,13 @@ int topk_distill(const thx_array* logits, const thx_array* teacher, const thx_ar
   set_last_plan(plan);
   if (dry || !in[0].rows) return THX_OK;
   if ((rc = ensure_init())) return rc;
-  return by_type(in[0].dtype, [&](auto t) {
+  return by_type(in[0].dtype, temperature, [&](auto t, auto fused) {
     typedef decltype(t) T;
+    constexpr bool FUSED = decltype(fused)::value;
     typedef typename AccOf<T>::type A;
     const KdRow<T> row = {teacher_args<A>(in[1], in[2]), (A)(1.0 / temperature), (A)(temperature * temperature),
                           (A*)out[0].ptr, (A*)out[1].ptr};
-    return launch_forward<T, false, false>(cut_of<T>(in[0], temperature, ws), row, plan);
+    return launch_forward<T, false, false>(cut_of<T, FUSED>(in[0], temperature, ws), row, plan);
   });
 }
 
@@ -1253,12 +1272,13 @@ int topk_distill_grad(const thx_array* logits, const thx_array* teacher, const t
   set_last_plan(plan);
   if (dry || !in[0].rows) return THX_OK;
   if ((rc = ensure_init())) return rc;
-  return by_type(in[0].dtype, [&](auto t) {
+  return by_type(in[0].dtype, temperature, [&](auto t, auto fused) {
     typedef decltype(t) T;
+    constexpr bool FUSED = decltype(fused)::value;
     typedef typename AccOf<T>::type A;
     const KdGrad<A> row = {teacher_args<A>(in[1], in[2]), (const A*)in[3].ptr, in[3].stride, (const A*)in[4].ptr,
                            in[4].stride, (A)(kLog2E / temperature), (A)temperature};
-    return launch_grad<T>(in[0], temperature, out, row, plan);
+    return launch_grad<T, FUSED>(in[0], temperature, out, row, plan);
   });
 }
 
@@ -1292,13 +1312,14 @@ int token_logprob_train(const thx_array* logits, const thx_array* tokens, const 
   set_last_plan(plan);
   if ((flags & THX_DRY_RUN) || !x.rows) return THX_OK;
   if ((rc = ensure_init())) return rc;
-  return by_type(x.dtype, [&](auto tag) {
+  return by_type(x.dtype, temperature, [&](auto tag, auto fused) {
     typedef decltype(tag) T;
+    constexpr bool FUSED = decltype(fused)::value;
     typedef typename AccOf<T>::type A;
     const LpTrain<T> row = {{t.ptr, t.stride, t.dtype == THX_I64, 0, (A)(1.0 / temperature),
                              {(A*)out[0].ptr, (A*)out[1].ptr, nullptr, nullptr, (A*)out[2].ptr}},
                             (const A*)gr.ptr, gr.stride, (const A*)ur.ptr, ur.stride};
-    return launch_train<T>(x, temperature, out[3], h, row, plan);
+    return launch_train<T, FUSED>(x, temperature, out[3], h, row, plan);
   });
 }
 
@@ -1328,13 +1349,14 @@ int topk_distill_train(const thx_array* logits, const thx_array* teacher, const 
   set_last_plan(plan);
   if ((flags & THX_DRY_RUN) || !x.rows) return THX_OK;
   if ((rc = ensure_init())) return rc;
-  return by_type(x.dtype, [&](auto tag) {
+  return by_type(x.dtype, temperature, [&](auto tag, auto fused) {
     typedef decltype(tag) T;
+    constexpr bool FUSED = decltype(fused)::value;
     typedef typename AccOf<T>::type A;
     const KdTrain<T> row = {{teacher_args<A>(t, ids), (A)(1.0 / temperature), (A)(temperature * temperature),
                              (A*)out[0].ptr, (A*)out[1].ptr},
                             (const A*)gr.ptr, gr.stride, (A)temperature};
-    return launch_train<T>(x, temperature, out[2], h, row, plan);
+    return launch_train<T, FUSED>(x, temperature, out[2], h, row, plan);
   });
 }
 
