@@ -394,9 +394,11 @@ THX_DEV void finish(const LpRow<T>& q, const T* x, int64_t cols, int64_t r, cons
     wave_fence();
     best.sort(k);
     if (lane < k) {
-      const int64_t j = key_column(best.list[lane]);
-      q.o.top_at[r * k + lane] = j;
-      q.o.top[r * k + lane] = none ? neg_inf<A>() : ex.log_prob((A)x[j], sum.m, q.inv_t, ls);
+      // there are k columns, and the list holds the k best: the look costs nothing, and no key becomes an address without it
+      const int64_t j = lane < best.n ? key_column(best.list[lane]) : cols;
+      const bool there = j < cols;
+      q.o.top_at[r * k + lane] = there ? j : -1;
+      q.o.top[r * k + lane] = !there ? (A)NAN : none ? neg_inf<A>() : ex.log_prob((A)x[j], sum.m, q.inv_t, ls);
     }
   }
 }
