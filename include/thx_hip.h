@@ -111,6 +111,12 @@ int thx_sync(void);
 void* thx_stream(void);
 int thx_check_device_pointer(const void* ptr);
 
+/* Order between that stream and another one (a hipStream_t of the library's device; null: its default stream) without a
+ * wait on the host: what is queued in the library's stream from now on runs after what `stream` holds now, and the other
+ * way round.  Both are refused while a recording is open: a replay would not repeat them. */
+int thx_wait_for_stream(void* stream);
+int thx_let_stream_wait(void* stream);
+
 /* ---- run-time compilation ----------------------------------------------- */
 
 /* Directory of the on-disk code-object cache (default $THX_CACHE_DIR, else

@@ -410,3 +410,14 @@ def test_views_of_other_libraries_arrays(dry_run):
             HipArray.from_cuda_array_interface(Other(**bad))
     assert HipArray.from_cuda_array_interface(Other(shape=(0, 4), data=(0, False))).shape == (0, 4)
     assert not hasattr(HipArray.empty((3,), "float32"), "__cuda_array_interface__")     # no memory behind it here
+
+
+def test_other_libraries_arrays_that_cannot_be_taken(dry_run):
+    class Other(object):
+        def __init__(self, **kw):
+            self.__cuda_array_interface__ = dict({"typestr": "<f4", "shape": (3,), "data": (1 << 20, False), "version": 3}, **kw)
+
+    for stream in (None, 1, 2, 1 << 30):
+        assert HipArray.from_cuda_array_interface(Other(stream=stream)).shape == (3,)
+    with pytest.raises(ValueError, match="ambiguous"):
+        HipArray.from_cuda_array_interface(Other(stream=0))

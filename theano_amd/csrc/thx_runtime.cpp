@@ -79,6 +79,8 @@ struct ProfRec {
 static bool g_profiling = false;
 static std::vector<ProfRec> g_prof;
 static hipEvent_t g_t0 = nullptr, g_t1 = nullptr;
+static hipEvent_t g_order = nullptr;  // between the library's stream and others; recorded anew for every wait
+static std::mutex g_order_mu;
 
 static int init_locked(int device) {
   Runtime& r = rt();
@@ -122,6 +124,7 @@ static int init_locked(int device) {
   THX_HIP_CHECK(hipStreamCreateWithFlags(&r.stream, hipStreamNonBlocking));
   THX_HIP_CHECK(hipEventCreate(&g_t0));
   THX_HIP_CHECK(hipEventCreate(&g_t1));
+  THX_HIP_CHECK(hipEventCreateWithFlags(&g_order, hipEventDisableTiming));
   r.ready = true;
   return THX_OK;
 }
@@ -694,6 +697,34 @@ int thx_check_device_pointer(const void* ptr) {
   if (attr.device != rt().device)
     return fail(THX_ERR_ARG, "%p lies on device %d, the library uses device %d", ptr, attr.device, rt().device);
   return THX_OK;
+}
+
+// What `then` holds from now on runs after what `first` holds now.  A null stream is the default one of the current device.
+static int order_streams(hipStream_t first, hipStream_t then) {
+  if (first == then) return THX_OK;
+  if (g_capturing) return fail(THX_ERR_ARG, "streams cannot be ordered while a recording is open: order them around its replays");
+  int current = -1;
+  THX_HIP_CHECK(hipGetDevice(&current));
+  if (current != rt().device) THX_HIP_CHECK(hipSetDevice(rt().device));
+  hipError_t e;
+  {
+    std::lock_guard<std::mutex> lk(g_order_mu);
+    e = hipEventRecord(g_order, first);
+    if (e == hipSuccess) e = hipStreamWaitEvent(then, g_order, 0);
+  }
+  if (current != rt().device) (void)hipSetDevice(current);
+  if (e != hipSuccess) return fail(THX_ERR_HIP, "streams could not be ordered: %s", hipGetErrorString(e));
+  return THX_OK;
+}
+
+int thx_wait_for_stream(void* stream) {
+  int rc = ensure_init();
+  return rc ? rc : order_streams((hipStream_t)stream, rt().stream);
+}
+
+int thx_let_stream_wait(void* stream) {
+  int rc = ensure_init();
+  return rc ? rc : order_streams(rt().stream, (hipStream_t)stream);
 }
 
 int thx_sync(void) {

@@ -1,6 +1,6 @@
 """HIP backend: runtime binding, device ops and the rewrites that lift a graph onto them."""
-from .runtime import (Graph, HipArray, HipRuntimeError, cache_stats, capture, device_info, dry_run, init, last_plan, profile,  # noqa: F401
-                      set_dry_run, stream, sync, timer_start, timer_stop)
+from .runtime import (Graph, HipArray, HipRuntimeError, cache_stats, capture, device_info, dry_run, init, last_plan, let_stream_wait,  # noqa: F401
+                      profile, set_dry_run, stream, sync, timer_start, timer_stop, wait_for_stream)
 from .ops import (HipArrayType, HipCAReduce, HipDimShuffle, HipElemwise, HipElemwiseReduce, HipMaxAndArgmax, HipToHost, HostToHip,  # noqa: F401
                   as_hip_variable,
                   hip_from_host, host_from_hip)

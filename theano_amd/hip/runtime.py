@@ -62,6 +62,8 @@ def _load():
         "thx_sync": ([], ctypes.c_int),
         "thx_stream": ([], vp),
         "thx_check_device_pointer": ([vp], ctypes.c_int),
+        "thx_wait_for_stream": ([vp], ctypes.c_int),
+        "thx_let_stream_wait": ([vp], ctypes.c_int),
         "thx_set_cache_dir": ([ctypes.c_char_p], ctypes.c_int),
         "thx_cache_stats": ([P(i64), P(i64), P(i64)], ctypes.c_int),
         "thx_elemwise_new": ([ctypes.c_char_p, ctypes.c_char_p, ctypes.c_int, ctypes.c_int, P(i32), P(vp)], ctypes.c_int),
@@ -188,6 +190,27 @@ def stream():
 
 
 _stream = None
+
+
+def wait_for_stream(other):
+    """What the library runs from now on waits, on the device, for what the stream ``other`` holds now: another library's
+    work on arguments, and on earlier results, whose memory is used again when they are let go.  ``other``: a
+    ``hipStream_t`` as an integer, 0 for the default stream (``torch.cuda.current_stream().cuda_stream``)."""
+    if not _initialised:
+        init()
+    rc = lib.thx_wait_for_stream(other)
+    if rc:
+        check(rc)
+
+
+def let_stream_wait(other):
+    """What the stream ``other`` holds from now on waits, on the device, for what the library has queued: another library's
+    work on results."""
+    if not _initialised:
+        init()
+    rc = lib.thx_let_stream_wait(other)
+    if rc:
+        check(rc)
 
 
 def last_plan():
@@ -446,10 +469,14 @@ class HipArray(object):
     @classmethod
     def from_cuda_array_interface(cls, obj):
         """A view of device memory that another library holds, through the ``__cuda_array_interface__`` protocol
-        (PyTorch tensors, CuPy arrays): nothing is copied, and ``obj`` lives as long as the view.  The counterpart of
-        ``pygpu.gpuarray.from_gpudata``.  The memory must be the library's device's.  Nothing is ordered here: work on
-        ``obj`` in another stream than ``stream()`` has to be finished, or ordered before that stream, when a function
-        is called on the view."""
+        (PyTorch tensors, CuPy arrays): nothing is copied, and ``obj`` lives as long as the view.  The counterpart of ``pygpu.gpuarray.from_gpudata``.
+        The memory must be the library's device's, and both libraries in one HIP runtime: import the other one (PyTorch,
+        which brings its own) before this package, which then uses the runtime that is there.
+
+        Where ``obj`` names the stream it is made in (the protocol's entry ``stream``), the library's further work waits
+        for that stream, on the device; while a recording is open such an array is refused.  Objects that name none
+        (PyTorch's) promise nothing: work on them in another stream than ``stream()`` has to be finished, or ordered by
+        ``wait_for_stream``, when a function is called on the view."""
         d = obj.__cuda_array_interface__
         if d.get("mask") is not None:
             raise TypeError("a masked array cannot be viewed as a HipArray")
@@ -462,6 +489,12 @@ class HipArray(object):
         if 0 in shape:
             return cls.empty(shape, dtype)
         strides = _c_strides_of(shape, dtype.itemsize) if strides is None else tuple(strides)
+        made_in = d.get("stream")
+        if made_in is not None:
+            if not made_in:
+                raise ValueError("the stream 0 of an array interface is ambiguous: 1 is the default stream, 2 the thread's own")
+            if not _dry:
+                wait_for_stream(0 if made_in == 1 else made_in)
         return cls._raw(_Foreign(obj, d["data"][0]), 0, shape, strides, dtype, code)
 
     @property
