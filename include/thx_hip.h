@@ -117,6 +117,12 @@ int thx_check_device_pointer(const void* ptr);
 int thx_wait_for_stream(void* stream);
 int thx_let_stream_wait(void* stream);
 
+/* A mark behind everything the library's stream holds now.  thx_mark_passed: *passed becomes 1 once the device has come to
+ * it, and the mark is freed with that; 0 until then.  For memory of other libraries that queued work still reads. */
+typedef struct thx_mark thx_mark;
+int thx_mark_set(thx_mark** out);
+int thx_mark_passed(thx_mark* mark, int* passed);
+
 /* ---- run-time compilation ----------------------------------------------- */
 
 /* Directory of the on-disk code-object cache (default $THX_CACHE_DIR, else

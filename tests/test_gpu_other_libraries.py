@@ -1,6 +1,8 @@
 """Arrays that pass between this library and other users of the device, which work in streams of their own: who waits for
-whom.  The other user here calls the HIP runtime directly."""
+whom, and how long memory stays.  The other user here calls the HIP runtime directly."""
 import ctypes
+import gc
+import weakref
 
 import numpy as np
 import pytest
@@ -125,9 +127,51 @@ def test_streams_ordered_by_the_caller(rt, plus_one):
     hip.wait_for_stream(hip.stream())                         # nothing to wait for
 
 
+def test_memory_stays_until_queued_work_has_ended(rt, plus_one):
+    hip.sync()
+    for n in (100, 20 << 20):                                 # one of many that share a mark, and one with its own
+        owner = Array(rt, n)
+        there = weakref.ref(owner)
+        rt.busy(hip.stream())
+        plus_one(HipArray.from_cuda_array_interface(owner))
+        del owner
+        gc.collect()
+        assert there() is not None
+        hip.sync()
+        assert there() is None
+    refs = []
+    for _ in range(100):
+        owner = Array(rt, 10)
+        refs.append(weakref.ref(owner))
+        plus_one(HipArray.from_cuda_array_interface(owner))
+        rt.sync()
+    del owner
+    assert sum(r() is not None for r in refs) <= 40           # let go on the way
+    hip.sync()
+    assert not any(r() is not None for r in refs)
+
+
 def test_recordings_and_other_libraries_arrays(rt, plus_one):
-    """A recording takes no array that has to be waited for."""
-    mine = Array(rt, 1000, value=2)
+    """A recording keeps what it reads, and takes no array that has to be waited for."""
+    owner = Array(rt, 1000)
+    mine = Array(rt, 1000, ptr=owner.ptr)                     # the same memory
+    there = weakref.ref(owner)
+    plus_one(HipArray.from_cuda_array_interface(owner))
+    with hip.capture() as c:
+        r = plus_one(HipArray.from_cuda_array_interface(owner))
+    del owner
+    hip.sync()
+    gc.collect()
+    assert there() is not None
+    for k in range(3):
+        rt.fill(mine, k, 0)
+        rt.sync()
+        c.graph.launch()
+        assert (r.to_numpy() == k + 1).all()
+    del c
+    gc.collect()
+    hip.sync()
+    assert there() is None
     with pytest.raises(ValueError, match="recording"):
         with hip.capture():
             HipArray.from_cuda_array_interface(Array(rt, 1000, stream=rt.stream(), ptr=mine.ptr))

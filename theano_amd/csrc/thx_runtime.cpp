@@ -12,6 +12,7 @@
 #include <cstring>
 #include <fstream>
 #include <mutex>
+#include <new>
 #include <sstream>
 #include <unordered_map>
 
@@ -725,6 +726,44 @@ int thx_wait_for_stream(void* stream) {
 int thx_let_stream_wait(void* stream) {
   int rc = ensure_init();
   return rc ? rc : order_streams(rt().stream, (hipStream_t)stream);
+}
+
+struct thx_mark {
+  hipEvent_t event;
+};
+
+int thx_mark_set(thx_mark** out) {
+  int rc = ensure_init();
+  if (rc) return rc;
+  if (!out) return fail(THX_ERR_ARG, "thx_mark_set: null argument");
+  if (g_capturing) return fail(THX_ERR_ARG, "thx_mark_set: a recording is open");
+  hipEvent_t event = nullptr;
+  THX_HIP_CHECK(hipEventCreateWithFlags(&event, hipEventDisableTiming));
+  hipError_t e = hipEventRecord(event, rt().stream);
+  thx_mark* m = e == hipSuccess ? new (std::nothrow) thx_mark : nullptr;
+  if (!m) {
+    (void)hipEventDestroy(event);
+    if (e != hipSuccess) return fail(THX_ERR_HIP, "thx_mark_set: %s", hipGetErrorString(e));
+    return fail(THX_ERR_MEMORY, "thx_mark_set: out of host memory");
+  }
+  m->event = event;
+  *out = m;
+  return THX_OK;
+}
+
+int thx_mark_passed(thx_mark* mark, int* passed) {
+  if (!mark || !passed) return fail(THX_ERR_ARG, "thx_mark_passed: null argument");
+  *passed = 0;
+  hipError_t e = hipEventQuery(mark->event);
+  if (e == hipErrorNotReady) {
+    (void)hipGetLastError();
+    return THX_OK;
+  }
+  if (e != hipSuccess) return fail(THX_ERR_HIP, "thx_mark_passed: %s", hipGetErrorString(e));
+  (void)hipEventDestroy(mark->event);
+  delete mark;
+  *passed = 1;
+  return THX_OK;
 }
 
 int thx_sync(void) {

@@ -6,6 +6,7 @@ when no device is present.  ``HipArray`` plays the role pygpu's ``GpuArray``
 plays for the reference (``theano/gpuarray/type.py:129-517``): a strided view
 (shape, byte strides, offset) over a reference-counted device buffer.
 """
+import collections
 import ctypes
 import functools
 import os
@@ -64,6 +65,8 @@ def _load():
         "thx_check_device_pointer": ([vp], ctypes.c_int),
         "thx_wait_for_stream": ([vp], ctypes.c_int),
         "thx_let_stream_wait": ([vp], ctypes.c_int),
+        "thx_mark_set": ([P(vp)], ctypes.c_int),
+        "thx_mark_passed": ([vp, P(ctypes.c_int)], ctypes.c_int),
         "thx_set_cache_dir": ([ctypes.c_char_p], ctypes.c_int),
         "thx_cache_stats": ([P(i64), P(i64), P(i64)], ctypes.c_int),
         "thx_elemwise_new": ([ctypes.c_char_p, ctypes.c_char_p, ctypes.c_int, ctypes.c_int, P(i32), P(vp)], ctypes.c_int),
@@ -177,6 +180,7 @@ def device_info():
 
 def sync():
     check(lib.thx_sync())
+    _release_passed(everything=True)
 
 
 def stream():
@@ -360,15 +364,63 @@ class _Buffer(object):
 
 
 class _Foreign(object):
-    """Device memory that another object owns."""
+    """Device memory that another object owns.  That object is kept beyond the last view of it, until the work that was
+    queued by then has ended: without that its library could hand the memory out again while kernels still read it."""
 
-    __slots__ = ("ptr", "owner", "fake")
+    __slots__ = ("ptr", "owner", "nbytes", "fake")
 
-    def __init__(self, owner, ptr):
-        self.ptr, self.owner, self.fake = ptr, owner, False
+    def __init__(self, owner, ptr, nbytes):
+        self.ptr, self.nbytes, self.fake = ptr, nbytes, False
+        self.owner = None
         if not _dry:
             init()
             check(lib.thx_check_device_pointer(ptr))
+        self.owner = owner
+        if _capture_keep is not None:
+            _capture_keep.append(self)
+
+    def __del__(self):
+        try:
+            owner, self.owner = self.owner, None
+            if owner is not None and not _dry:
+                _keep_for_queued_work(owner, self.nbytes)
+        except Exception:
+            pass
+
+
+# Owners of memory whose last view is gone: those let go since the last mark in the library's stream, and behind a mark
+# each the ones before.  A mark costs a few microseconds, so that small arrays share one.
+_MARK_OWNERS, _MARK_BYTES = 16, 64 << 20
+_let_go, _let_go_bytes = [], 0
+_marked = collections.deque()
+
+
+def _keep_for_queued_work(owner, nbytes):
+    global _let_go, _let_go_bytes
+    if _capture_keep is not None:       # what the open recording has taken in may read it with every replay
+        _capture_keep.append(owner)
+        return
+    _let_go.append(owner)
+    _let_go_bytes += nbytes
+    if len(_let_go) >= _MARK_OWNERS or _let_go_bytes >= _MARK_BYTES:
+        mark = ctypes.c_void_p()
+        check(lib.thx_mark_set(ctypes.byref(mark)))
+        owners, _let_go, _let_go_bytes = _let_go, [], 0
+        _marked.append((mark, owners))
+        _release_passed()
+
+
+def _release_passed(everything=False):
+    """Lets go of the owners whose mark the device has passed; ``everything``: the stream has just been waited for."""
+    global _let_go, _let_go_bytes
+    passed = ctypes.c_int()
+    while _marked:
+        check(lib.thx_mark_passed(_marked[0][0], ctypes.byref(passed)))
+        if not passed.value:
+            break
+        _marked.popleft()
+    if everything and not _marked:
+        _let_go, _let_go_bytes = [], 0
 
 
 def _c_strides(shape, itemsize):
@@ -469,7 +521,8 @@ class HipArray(object):
     @classmethod
     def from_cuda_array_interface(cls, obj):
         """A view of device memory that another library holds, through the ``__cuda_array_interface__`` protocol
-        (PyTorch tensors, CuPy arrays): nothing is copied, and ``obj`` lives as long as the view.  The counterpart of ``pygpu.gpuarray.from_gpudata``.
+        (PyTorch tensors, CuPy arrays): nothing is copied, and ``obj`` lives as long as the view and the work that was
+        queued on it (which later imports and ``sync()`` look for).  The counterpart of ``pygpu.gpuarray.from_gpudata``.
         The memory must be the library's device's, and both libraries in one HIP runtime: import the other one (PyTorch,
         which brings its own) before this package, which then uses the runtime that is there.
 
@@ -495,7 +548,10 @@ class HipArray(object):
                 raise ValueError("the stream 0 of an array interface is ambiguous: 1 is the default stream, 2 the thread's own")
             if not _dry:
                 wait_for_stream(0 if made_in == 1 else made_in)
-        return cls._raw(_Foreign(obj, d["data"][0]), 0, shape, strides, dtype, code)
+        nbytes = dtype.itemsize
+        for s in shape:
+            nbytes *= s
+        return cls._raw(_Foreign(obj, d["data"][0], nbytes), 0, shape, strides, dtype, code)
 
     @property
     def __cuda_array_interface__(self):
