@@ -11,6 +11,7 @@ import theano_amd as th
 from theano_amd import hip, tensor as T
 from theano_amd.compile import Out
 from theano_amd.hip.runtime import HipArray
+from theano_amd.tensor import inplace
 
 pytestmark = pytest.mark.gpu
 
@@ -179,3 +180,15 @@ def test_recordings_and_other_libraries_arrays(rt, plus_one):
         r = plus_one(HipArray.from_cuda_array_interface(Array(rt, 1000, stream=hip.stream(), ptr=mine.ptr)))
     c.graph.launch()
     assert (r.to_numpy() == 3).all()
+
+
+def test_arrays_that_a_function_overwrites(rt):
+    x, y = T.fvector(), T.fvector()
+    f = th.function([x, y], inplace.add_inplace(x, y), accept_inplace=True)
+    t = Array(rt, 10)
+    u, fixed = Array(rt, 10, value=1, read_only=True), Array(rt, 10, ptr=t.ptr, read_only=True)
+    with pytest.raises(ValueError, match="read-only"):
+        f(HipArray.from_cuda_array_interface(fixed), HipArray.from_cuda_array_interface(u))
+    f(HipArray.from_cuda_array_interface(t), HipArray.from_cuda_array_interface(u))
+    hip.sync()
+    assert (rt.read(t) == 1).all() and (rt.read(u) == 1).all()

@@ -421,3 +421,10 @@ def test_other_libraries_arrays_that_cannot_be_taken(dry_run):
         assert HipArray.from_cuda_array_interface(Other(stream=stream)).shape == (3,)
     with pytest.raises(ValueError, match="ambiguous"):
         HipArray.from_cuda_array_interface(Other(stream=0))
+    from theano_amd.tensor import inplace
+    x, y = T.fvector(), T.fvector()
+    f = th.function([x, y], inplace.add_inplace(x, y), accept_inplace=True)
+    plain, fixed = [HipArray.from_cuda_array_interface(Other(data=(1 << 20, ro))) for ro in (False, True)]
+    f(plain, fixed)
+    with pytest.raises(ValueError, match="read-only"):
+        f(fixed, plain)

@@ -346,6 +346,9 @@ class Function(object):
         if not self._constants_ready:
             self._upload_constants()
         HipArray = self._HipArray
+        for k in self.writeback:
+            if isinstance(args[k], HipArray) and getattr(args[k].buffer, "read_only", False):
+                raise ValueError("argument %d (%s) would be overwritten, and its memory is read-only" % (k, self.in_specs[k].name))
         for spec, var, a in zip(self.in_specs, self.fgraph.inputs, args):
             if type(a) is np.ndarray and a.dtype == var.type.numpy_dtype and a.shape == self._last_shape.get(var):
                 self.storage[var][0] = a  # same dtype and shape as a value that already passed the full check

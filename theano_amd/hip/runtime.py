@@ -367,10 +367,10 @@ class _Foreign(object):
     """Device memory that another object owns.  That object is kept beyond the last view of it, until the work that was
     queued by then has ended: without that its library could hand the memory out again while kernels still read it."""
 
-    __slots__ = ("ptr", "owner", "nbytes", "fake")
+    __slots__ = ("ptr", "owner", "nbytes", "read_only", "fake")
 
-    def __init__(self, owner, ptr, nbytes):
-        self.ptr, self.nbytes, self.fake = ptr, nbytes, False
+    def __init__(self, owner, ptr, nbytes, read_only):
+        self.ptr, self.nbytes, self.read_only, self.fake = ptr, nbytes, read_only, False
         self.owner = None
         if not _dry:
             init()
@@ -529,7 +529,8 @@ class HipArray(object):
         Where ``obj`` names the stream it is made in (the protocol's entry ``stream``), the library's further work waits
         for that stream, on the device; while a recording is open such an array is refused.  Objects that name none
         (PyTorch's) promise nothing: work on them in another stream than ``stream()`` has to be finished, or ordered by
-        ``wait_for_stream``, when a function is called on the view."""
+        ``wait_for_stream``, when a function is called on the view.  Functions write to their arguments only where the
+        graph says so (``accept_inplace``), and refuse memory that ``obj`` calls read-only then."""
         d = obj.__cuda_array_interface__
         if d.get("mask") is not None:
             raise TypeError("a masked array cannot be viewed as a HipArray")
@@ -548,10 +549,11 @@ class HipArray(object):
                 raise ValueError("the stream 0 of an array interface is ambiguous: 1 is the default stream, 2 the thread's own")
             if not _dry:
                 wait_for_stream(0 if made_in == 1 else made_in)
+        ptr, read_only = d["data"]
         nbytes = dtype.itemsize
         for s in shape:
             nbytes *= s
-        return cls._raw(_Foreign(obj, d["data"][0], nbytes), 0, shape, strides, dtype, code)
+        return cls._raw(_Foreign(obj, ptr, nbytes, read_only), 0, shape, strides, dtype, code)
 
     @property
     def __cuda_array_interface__(self):
