@@ -367,10 +367,10 @@ class _Foreign(object):
     """Device memory that another object owns.  That object is kept beyond the last view of it, until the work that was
     queued by then has ended: without that its library could hand the memory out again while kernels still read it."""
 
-    __slots__ = ("ptr", "owner", "nbytes", "read_only", "fake")
+    __slots__ = ("ptr", "owner", "shape", "itemsize", "read_only", "fake")
 
-    def __init__(self, owner, ptr, nbytes, read_only):
-        self.ptr, self.nbytes, self.read_only, self.fake = ptr, nbytes, read_only, False
+    def __init__(self, owner, ptr, shape, itemsize, read_only):
+        self.ptr, self.shape, self.itemsize, self.read_only, self.fake = ptr, shape, itemsize, read_only, False
         self.owner = None
         if not _dry:
             init()
@@ -381,32 +381,39 @@ class _Foreign(object):
 
     def __del__(self):
         try:
-            owner, self.owner = self.owner, None
-            if owner is not None and not _dry:
-                _keep_for_queued_work(owner, self.nbytes)
+            owner = self.owner
+            if owner is not None and (_capture_keep is not None or id(owner) not in _let_go):
+                _keep_for_queued_work(owner, self.shape, self.itemsize)
         except Exception:
             pass
 
 
-# Owners of memory whose last view is gone: those let go since the last mark in the library's stream, and behind a mark
-# each the ones before.  A mark costs a few microseconds, so that small arrays share one.
-_MARK_OWNERS, _MARK_BYTES = 16, 64 << 20
-_let_go, _let_go_bytes = [], 0
+# Owners of memory whose last view is gone, by identity: those let go since the last mark in the library's stream, and
+# behind a mark each the ones before.  A mark between two kernels costs the device some 4 us, so that many arrays share
+# one, and an owner that comes with every call (inputs kept by the caller) counts once.
+_MARK_OWNERS, _MARK_BYTES = 64, 1 << 30
+_let_go, _let_go_bytes = {}, 0
 _marked = collections.deque()
 
 
-def _keep_for_queued_work(owner, nbytes):
+def _keep_for_queued_work(owner, shape, itemsize):
     global _let_go, _let_go_bytes
+    if _dry:
+        return
     if _capture_keep is not None:       # what the open recording has taken in may read it with every replay
         _capture_keep.append(owner)
         return
-    _let_go.append(owner)
+    nbytes = itemsize
+    for s in shape:
+        nbytes *= s
+    _let_go[id(owner)] = owner
     _let_go_bytes += nbytes
     if len(_let_go) >= _MARK_OWNERS or _let_go_bytes >= _MARK_BYTES:
         mark = ctypes.c_void_p()
         check(lib.thx_mark_set(ctypes.byref(mark)))
-        owners, _let_go, _let_go_bytes = _let_go, [], 0
+        owners, _let_go, _let_go_bytes = _let_go, {}, 0
         _marked.append((mark, owners))
+        del owners
         _release_passed()
 
 
@@ -420,7 +427,7 @@ def _release_passed(everything=False):
             break
         _marked.popleft()
     if everything and not _marked:
-        _let_go, _let_go_bytes = [], 0
+        _let_go, _let_go_bytes = {}, 0
 
 
 def _c_strides(shape, itemsize):
@@ -550,10 +557,7 @@ class HipArray(object):
             if not _dry:
                 wait_for_stream(0 if made_in == 1 else made_in)
         ptr, read_only = d["data"]
-        nbytes = dtype.itemsize
-        for s in shape:
-            nbytes *= s
-        return cls._raw(_Foreign(obj, ptr, nbytes, read_only), 0, shape, strides, dtype, code)
+        return cls._raw(_Foreign(obj, ptr, shape, dtype.itemsize, read_only), 0, shape, strides, dtype, code)
 
     @property
     def __cuda_array_interface__(self):
