@@ -257,11 +257,22 @@ _OUTPUTS = {"ln_forward": ("y",), "ln_train": ("y", "dx", "dgamma", "dbeta"),
             "kd_train": ("loss", "dlogits")}
 
 
+@functools.lru_cache(maxsize=None)
+def _one_stream():
+    """From here on torch works in the library's stream, as a program that uses both keeps it: calls run in their order,
+    and neither waits for the other."""
+    from theano_amd import hip
+    stream = torch.cuda.ExternalStream(hip.stream())
+    stream.wait_stream(torch.cuda.current_stream())
+    torch.cuda.set_stream(stream)
+
+
 def _own(s):
-    from theano_amd.hip import HipArray
+    from theano_amd import hip
     case = s["case"]
     f = _compiled(case["op"], case["dtype"], case.get("params"), case.get("top"), case.get("temperature"))
-    results = f(*[HipArray.from_cuda_array_interface(s[name]) for name in _INPUTS[case["op"]]])
+    _one_stream()
+    results = f(*[hip.HipArray.from_cuda_array_interface(s[name]) for name in _INPUTS[case["op"]]])
     return {name: torch.as_tensor(r, device="cuda") for name, r in zip(_OUTPUTS[case["op"]], results)}
 
 
