@@ -669,6 +669,38 @@ def test_entries_that_name_the_same_columns(entries):
 
 # ---- gradients against differences, and the operators together ---------------------------------------------
 
+@pytest.mark.parametrize("pdtype", [None, "float16", "float32"])
+@pytest.mark.parametrize("stats", [(True, False), (False, True), (True, True)])
+def test_gradients_through_statistics_are_rounded_once(pdtype, stats):
+    """dx of float16 rows is the sum of what arrives through the result and through the statistics, rounded once: half a
+    step of the sum, whatever the size of its parts."""
+    rng = np.random.default_rng(31)
+    shape = (60, 333)
+    x, dy = [rng.standard_normal(shape).astype("float16") for _ in range(2)]
+    gamma, beta = [rng.standard_normal(333).astype(pdtype or "float16") for _ in range(2)]
+    # of the size of dx in each element, so that parts cancel
+    dmean, dinv = [(333 * rng.standard_normal(60) * there).astype("float32") for there in stats]
+    xt, dyt, mt, it = tensor("float16", 2), tensor("float16", 2), T.fvector(), T.fvector()
+    ps = [tensor(pdtype, 1) for _ in range(2)] if pdtype else []
+    y, mean, inv = T.nnet.layer_normalization(xt, *ps)
+    known = {y: dyt}
+    known.update((v, g) for v, g, there in ((mean, mt, stats[0]), (inv, it, stats[1])) if there)
+    f = th.function([xt, dyt, mt, it] + ps, th.grad(None, [xt] + ps, known_grads=known), on_unused_input="ignore")
+    got = f(x, dy, dmean, dinv, *([gamma, beta] if pdtype else []))
+    ref = ln_ref(x, gamma if pdtype else None, beta if pdtype else None, 1e-5, dy)
+    m, i = ref["mean"][0][:, None], ref["invstd"][0][:, None]
+    parts = [dmean[:, None] / 333.0, -dinv[:, None] * i ** 3 / 333.0 * (x.astype("float64") - m)]
+    value = ref["dx"][0] + parts[0] + parts[1]
+    # x - mean is off by roundings of the largest |x|, and of invstd the cube is taken
+    big = np.abs(x.astype("float64")).max(-1, keepdims=True)
+    scale = ref["dx"][1] + np.abs(parts[0]) + 4 * np.abs(dinv[:, None]) * (ref["invstd"][1][:, None]) ** 3 / 333.0 * 2 * big
+    close(got[0], value, scale, chain(333), "dx", "float32")
+    if pdtype:
+        for g, name in zip(got[1:], ("dgamma", "dbeta")):
+            assert str(g.dtype) == pdtype
+            close(g, *ref[name], chain(333, 60), name, "float32")
+
+
 def differences(f, args, k, h):
     """Central differences of the scalar function ``f`` with respect to its argument ``k``."""
     out = np.zeros(args[k].shape)

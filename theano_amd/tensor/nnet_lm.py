@@ -96,14 +96,19 @@ class LayerNormalization(Op):
         x, params = inputs[0], inputs[1:]
         _, mean, invstd = outputs
         dy, dmean, dinvstd = grads
+        acc = mean.type.dtype
         if _is_zero(dy):
             res = [None] * len(inputs)
         else:
-            res = list(LayerNormalizationGrad(len(params))(x, dy, mean, invstd, *params[:1], return_list=True))
+            args = [x, dy] + params[:1]
+            if x.type.dtype != acc and not (_is_zero(dmean) and _is_zero(dinvstd)):
+                args = [T.cast(v, acc) for v in args]       # dx is added to below, and rounded behind that
+            res = list(LayerNormalizationGrad(len(params))(*(args[:2] + [mean, invstd] + args[2:]), return_list=True))
+            res[1:] = [r if r.type.dtype == p.type.dtype else T.cast(r, p.type.dtype) for r, p in zip(res[1:], params)]
         # what arrives through the statistics: d mean / dx = 1 / n, d invstd / dx = -invstd^3 (x - mean) / n
         nd = x.type.ndim
         col = list(range(nd - 1)) + ["x"]
-        n = T.ShapeFloat(nd - 1, mean.type.dtype)(x)
+        n = T.ShapeFloat(nd - 1, acc)(x)
         extra = None
         if not _is_zero(dmean):
             extra = T.second(x, (dmean / n).dimshuffle(*col))
@@ -111,8 +116,7 @@ class LayerNormalization(Op):
             term = (-dinvstd * invstd ** 3 / n).dimshuffle(*col) * (x - mean.dimshuffle(*col))
             extra = term if extra is None else extra + term
         if extra is not None:
-            extra = T.cast(extra, x.type.dtype)
-            res[0] = extra if res[0] is None else res[0] + extra
+            res[0] = T.cast(extra if res[0] is None else res[0] + extra, x.type.dtype)
         return [_disconnected() if r is None else r for r in res]
 
     def connection_pattern(self, node):
