@@ -36,7 +36,8 @@ struct Rows {
 };
 
 // Takes `a` apart into rows: the last `trailing` (0 or 1) axes are the columns, the axes before them have to collapse
-// to one stride.  `dtype` < 0: any (the caller looks at it).  `unit`: columns lie side by side.
+// to one stride.  `dtype` < 0: any (the caller looks at it).  Columns have to lie side by side (THX_ERR_UNSUPPORTED
+// otherwise, as for rows at more than one stride).
 inline int rows_of(const char* what, const char* name, const thx_array* a, int dtype, int trailing, int flags, Rows* r) {
   if (!a) return fail(THX_ERR_ARG, "%s: %s is missing", what, name);
   if (a->nd < trailing || a->nd > THX_MAX_ND)
