@@ -346,8 +346,8 @@ def token_log_probs(logits, tokens, n_top=0, temperature=1.0):
 
     Results are float32 (float64 for float64 logits).  All three floating-point results carry a gradient to the logits.
 
-    A logit of -infinity is a token that cannot occur: probability and gradient 0, log probability -infinity.  A row of
-    nothing else has log probabilities of -infinity, an entropy of 0 and no gradient.  A negative token stands for none
+    A logit of -infinity is a token that cannot occur: probability 0, log probability -infinity, and a gradient of 0 unless
+    it is the row's given token (or among its alternatives), whose own weight it gets.  A row of nothing else has log probabilities of -infinity, an entropy of 0 and no gradient.  A negative token stands for none
     (padding): ``log_prob`` 0, no gradient through it.  A token beyond the last column makes its row's ``log_prob`` NaN,
     and the row's gradient where the one of ``log_prob`` is asked for.  NaN or +infinity among a row's logits make its
     floating-point results and its gradient NaN."""
