@@ -1,9 +1,10 @@
 // Device code of waves of 64 lanes, run on the host: every lane is a context of its own that runs until it reaches an
 // operation of the whole wave (a ballot, a permutation, a fence) or of its block (a barrier), and goes on once all lanes
 // have reached the same one.  Between two of them the lanes run one after the other, so what one lane leaves in LDS for
-// another without a fence between comes out wrong, and lanes that part ways end the program.  Compiled with an address
-// checker, every access outside its array does too.
+// another without a fence between comes out wrong, and lanes that part ways end the program.  Compiled with
+// AddressSanitizer, every access outside its array does too.
 #pragma once
+
 #include <algorithm>
 #include <cmath>
 #include <cstdint>

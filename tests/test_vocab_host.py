@@ -1,4 +1,4 @@
-"""The kernels over a vocabulary, compiled for the host with an address checker and run lane by lane: what they read and
+"""The kernels over a vocabulary, compiled for the host with AddressSanitizer and run lane by lane: what they read and
 write lies inside the arrays they are given, lanes stay together where the wave acts as one, and the best columns are
 those of a sort."""
 import os
