@@ -700,13 +700,25 @@ int thx_check_device_pointer(const void* ptr) {
   return THX_OK;
 }
 
-// What `then` holds from now on runs after what `first` holds now.  A null stream is the default one of the current device.
+// The library's device as the current one, for as long as this lives: events and default streams belong to that.
+struct OnDevice {
+  int was = -1;
+  hipError_t error;
+  OnDevice() {
+    error = hipGetDevice(&was);
+    if (error == hipSuccess && was != rt().device) error = hipSetDevice(rt().device);
+  }
+  ~OnDevice() {
+    if (was >= 0 && was != rt().device) (void)hipSetDevice(was);
+  }
+};
+
+// What `then` holds from now on runs after what `first` holds now.  A null stream is the default one.
 static int order_streams(hipStream_t first, hipStream_t then) {
   if (first == then) return THX_OK;
   if (g_capturing) return fail(THX_ERR_ARG, "streams cannot be ordered while a recording is open: order them around its replays");
-  int current = -1;
-  THX_HIP_CHECK(hipGetDevice(&current));
-  if (current != rt().device) THX_HIP_CHECK(hipSetDevice(rt().device));
+  OnDevice device;
+  THX_HIP_CHECK(device.error);
   // an idle stream holds nothing to wait for; a wait costs the device some 20 us, the question the host 1
   hipError_t e = hipStreamQuery(first);
   if (e == hipErrorNotReady) {
@@ -715,7 +727,6 @@ static int order_streams(hipStream_t first, hipStream_t then) {
     e = hipEventRecord(g_order, first);
     if (e == hipSuccess) e = hipStreamWaitEvent(then, g_order, 0);
   }
-  if (current != rt().device) (void)hipSetDevice(current);
   if (e != hipSuccess) return fail(THX_ERR_HIP, "streams could not be ordered: %s", hipGetErrorString(e));
   return THX_OK;
 }
@@ -739,6 +750,8 @@ int thx_mark_set(thx_mark** out) {
   if (rc) return rc;
   if (!out) return fail(THX_ERR_ARG, "thx_mark_set: null argument");
   if (g_capturing) return fail(THX_ERR_ARG, "thx_mark_set: a recording is open");
+  OnDevice device;
+  THX_HIP_CHECK(device.error);
   hipEvent_t event = nullptr;
   THX_HIP_CHECK(hipEventCreateWithFlags(&event, hipEventDisableTiming));
   hipError_t e = hipEventRecord(event, rt().stream);
